@@ -29,6 +29,11 @@ INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 HIPCC = "/opt/rocm/bin/hipcc"
 ARCH = "gfx950"
 
+# No v_pk_add/mul/fma_f32 anywhere: hipcc forms them from plain float code by
+# itself, and some of their forms have returned wrong values on this part.
+# (hipcc's host pass warns that it does not know the feature; harmless.)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 # Per-file flags.  The word<->region kernels interleave f32 VALU with MFMAs by
 # hand: SLP vectorisation would pack adjacent f32 adds/multiplies into
 # v_pk_*_f32, which cost more than two plain ops beside MFMAs
@@ -98,7 +103,8 @@ def _build_locked(verbose, extra):
     digest = source_hash(tuple(extra))
     os.makedirs(OBJ_DIR, exist_ok=True)
     common = [HIPCC, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
-              "-fno-gpu-rdc", "-Wno-unused-result", "-Wno-unused-value", "-I", CSRC, *extra]
+              "-fno-gpu-rdc", "-Wno-unused-result", "-Wno-unused-value",
+              *NO_PACKED_FP32, "-I", CSRC, *extra]
     if verbose:
         common.append("-Rpass-analysis=kernel-resource-usage")
     jobs = []
