@@ -808,6 +808,66 @@ int tgfr_fcfm_conv_dw(const float* x, long long s_b, long long s_p, const float*
                       const int8_t* code, int B, float* dW, float* db, float* ws, int mode,
                       void* stream);
 
+/* Cross attention to an encoder's states of another length, H query heads on
+ * Hk key heads (H a multiple of Hk; head h reads key head h / (H / Hk)), D <=
+ * 256 columns: the general form of the fusion attention of
+ * models/fusion_nets.py:93-118, whose x and y share one H*W.
+ *   O[b,i,h] = sum_j P_ij V[b,j],  P = softmax_j(scale Q K^T)
+ * over the states j < kv_lens[b] with mask[b * mask_sb + j] != 0 (NULL: all).
+ * Rows i >= q_lens[b], and rows without a kept state, are zero.  Lengths are
+ * clamped to [0, Tq] / [0, Tk].  What masked states hold (NaN, infinity) has
+ * no effect.
+ *   type: 0 = bf16, 1 = fp32, 2 = fp16 tensors.
+ *   strides (host memory): 3 per tensor, over samples, tokens and heads, in
+ * elements, in the order of the tensor arguments; the last axis is dense.
+ * Any alignment of the element is read and written.
+ *   lse [B][Hk][Tq H / Hk] (forward: may be NULL): the rows' statistics for
+ * the backward.  scale > 0.
+ *   ws: tgfr_cross_attention_ws floats (forward: NULL where that is 0).
+ * The backward gives dq, dk, dv of the same type (dk, dv: both or neither),
+ * all overwritten; those of masked and padded places are zero.  Sums run in a
+ * fixed order: equal calls give equal bits. */
+int tgfr_cross_attention_ws(int B, int Tq, int Tk, int H, int Hk, int D, int type, int backward,
+                            long long* floats);
+int tgfr_cross_attention_fwd(const void* q, const void* k, const void* v, void* o,
+                             const long long* strides, const int* q_lens, const int* kv_lens,
+                             const uint8_t* mask, long long mask_sb, int B, int Tq, int Tk, int H,
+                             int Hk, int D, float scale, int type, float* lse, float* ws,
+                             void* stream);
+int tgfr_cross_attention_bwd(const void* q, const void* k, const void* v, const void* o,
+                             const void* dout, void* dq, void* dk, void* dv,
+                             const long long* strides, const int* q_lens, const int* kv_lens,
+                             const uint8_t* mask, long long mask_sb, int B, int Tq, int Tk, int H,
+                             int Hk, int D, float scale, int type, const float* lse, float* ws,
+                             void* stream);
+
+/* RMS norm of each head of the queries and keys with the position rotation in
+ * the same pass: n = x rsqrt(mean x^2 + eps), u = n w, and the R / 2 first
+ * pairs of u (elements i and i + R / 2, or 2 i and 2 i + 1 when interleaved)
+ * turned by pos * turn[i] / 2^64 of a circle; the D - R elements behind them
+ * are normed only.  D even, <= 256; q and k may each be NULL (not both).
+ *   shapes (host memory), 15 per part (q, k): B, T, H; strides over samples,
+ * tokens and heads of x, of dy (backward), and of y (backward: dx); strides
+ * over samples, tokens and axes of the positions.
+ *   qpos / kpos: int32 (pos32) or int64 positions, NULL: 0 .. T - 1 on every
+ * axis.  turn [R / 2]: fractions of a circle per position step, times 2^64;
+ * pair i follows axis i / (R / 2 / axes).
+ *   type_in of q and k, type_out of yq and yk: equal, or fp32 to bf16 / fp16.
+ * The backward gives dq, dk (type_in) and, with ws (tgfr_qk_norm_rope_ws
+ * floats), dwq, dwk [D] (each may be NULL). */
+int tgfr_qk_norm_rope_ws(int D, long long* floats);
+int tgfr_qk_norm_rope_fwd(const void* q, const void* k, void* yq, void* yk, const long long* shapes,
+                          const float* wq, const float* wk, const void* qpos, const void* kpos,
+                          int pos32, const unsigned long long* turn, int R, int axes,
+                          int interleaved, int D, float eps, int type_in, int type_out,
+                          void* stream);
+int tgfr_qk_norm_rope_bwd(const void* q, const void* k, const void* dyq, const void* dyk, void* dq,
+                          void* dk, const long long* shapes, const float* wq, const float* wk,
+                          const void* qpos, const void* kpos, int pos32,
+                          const unsigned long long* turn, int R, int axes, int interleaved, int D,
+                          float eps, int type_in, int type_out, float* ws, float* dwq, float* dwk,
+                          void* stream);
+
 #ifdef __cplusplus
 }
 #endif

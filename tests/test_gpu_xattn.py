@@ -1,0 +1,553 @@
+"""Cross attention (csrc/tgfr_xattn.h) and the query / key norm with rotation
+(csrc/tgfr_rope.hip) against their formulas in 64 bits.
+
+Tolerances are bounds, element by element, from the roundings that the kernels
+make: u is half a step of the tensors' type (the result; P and dS as matrix
+operands), e the fp32 arithmetic: a sum of n products is off by at most
+(n + 8) 2^-24 of the sum of their magnitudes, and a probability by twice the
+error of its score (as an exponent) and the error of its row's sum."""
+import math
+from decimal import Decimal, getcontext
+
+import pytest
+import torch
+
+from text_guided_face_recognition_amd import kernels as K
+
+pytestmark = pytest.mark.gpu
+
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+U32 = 2.0 ** -24
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def heads(x, n):
+    """[B, T, Hk, D] -> [B, H, T, D] of the query heads, in 64 bits."""
+    return x.double().repeat_interleave(n // x.shape[2], 2).transpose(1, 2)
+
+
+def formula(q, k, v, do, scale, keep):
+    """o, dq, dk, dv of the formulas in 64 bits and the bounds of their errors.
+    keep [B, 1 or H, Tq, Tk]: what is attended to."""
+    u, h, hk, d = half_step(q.dtype), q.shape[2], k.shape[2], q.shape[3]
+    f16 = q.dtype == F16
+    out, tol = {}, {}
+    kz = torch.where(keep.any(-2).any(1)[:, :, None, None], k, 0)
+    vz = torch.where(keep.any(-2).any(1)[:, :, None, None], v, 0)
+    live = keep.any(-1).any(1)[:, :, None, None]
+    qz, doz = torch.where(live, q, 0), torch.where(live, do, 0)
+    Q, KK, V, DO = heads(qz, h), heads(kz, h), heads(vz, h), heads(doz, h)
+    tk, rows = KK.shape[2], Q.shape[2] * (h // hk)
+    s = scale * Q @ KK.transpose(2, 3)
+    s_err = (d + 8) * U32 * (scale * Q.abs() @ KK.abs().transpose(2, 3)).amax().item() + \
+        4 * U32 * s.abs().amax().item()
+    s = s.masked_fill(~keep, -math.inf)
+    top = s.amax(-1, keepdim=True)
+    e = torch.exp(s - torch.where(top.isinf(), 0.0, top))
+    z = e.sum(-1, keepdim=True)
+    P = e / torch.where(z == 0, 1.0, z)
+    p_err = 4 * s_err + (tk + 40) * U32                         # relative
+    tiny = 2.0 ** -24 if f16 else 0.0                           # fp16: P, dS below its range
+    O = P @ V
+    o_tol = u * O.abs() + (u + p_err + (tk + 8) * U32) * (P @ V.abs()) + \
+        tiny * V.abs().sum(2, keepdim=True)
+    dP = DO @ V.transpose(2, 3)
+    delta = (DO * O).sum(-1, keepdim=True)
+    dP_mag, dl_mag = DO.abs() @ V.abs().transpose(2, 3), (DO * O).abs().sum(-1, keepdim=True)
+    dS = P * (dP - delta)
+    ds_err = P * ((d + 8) * U32 * (dP_mag + dl_mag) + (DO.abs() * o_tol).sum(-1, keepdim=True)) + \
+        (u + p_err + 8 * U32) * dS.abs()
+    row_max = DO.abs().amax(-1, keepdim=True)
+    ds_err_q = ds_err + 2 * tiny * row_max
+    ds_err_k = ds_err + 2 * tiny * row_max.amax((1, 2), keepdim=True)
+    dQ = scale * dS @ KK
+    dq_tol = u * dQ.abs() + scale * (ds_err_q + (tk + 8) * U32 * dS.abs()) @ KK.abs()
+
+    def shared(x):               # [B, H, Tk, D] -> [B, Tk, Hk, D], summed over shared heads
+        return x.view(x.shape[0], hk, h // hk, *x.shape[2:]).sum(2).transpose(1, 2)
+    PT, ST = P.transpose(2, 3), dS.transpose(2, 3)
+    dK, dV = shared(scale * ST @ Q), shared(PT @ DO)
+    dk_tol = u * dK.abs() + shared(
+        scale * (ds_err_k.transpose(2, 3) + (rows + 8) * U32 * ST.abs()) @ Q.abs())
+    dv_tol = u * dV.abs() + shared(
+        ((u + p_err + (rows + 8) * U32) * PT + tiny) @ DO.abs())
+    for n, x, t in (("o", O.transpose(1, 2), o_tol.transpose(1, 2)),
+                    ("dq", dQ.transpose(1, 2), dq_tol.transpose(1, 2)), ("dk", dK, dk_tol),
+                    ("dv", dV, dv_tol)):
+        out[n], tol[n] = x, t + (1e-30 if not f16 else 2.0 ** -25)
+    return out, tol
+
+
+def keep_of(b, tq, tk, q_lens=None, kv_lens=None, mask=None):
+    keep = torch.ones(b, 1, tq, tk, dtype=torch.bool, device="cuda")
+    if kv_lens is not None:
+        keep &= (torch.arange(tk, device="cuda") < kv_lens.view(b, 1, 1, 1))
+    if mask is not None:
+        keep &= mask.view(b, 1, 1, tk)
+    if q_lens is not None:
+        keep &= (torch.arange(tq, device="cuda").view(1, 1, tq, 1) < q_lens.view(b, 1, 1, 1))
+    return keep
+
+
+def randn(g, *shape, dtype):
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+def within(got, want, tol, name):
+    off = (got.double() - want).abs()
+    assert bool(torch.isfinite(got).all()), f"{name} is not finite"
+    worst = (off - tol).max().item()
+    assert worst <= 0, f"{name}: {off.max().item():.3g} off, {worst:.3g} over the bound"
+
+
+def check(q, k, v, do, scale=None, q_lens=None, kv_lens=None, mask=None):
+    """Forward, backward, and the forward that keeps no statistics."""
+    q, k, v = (x.detach().requires_grad_() for x in (q, k, v))
+    kw = dict(scale=scale, q_lens=q_lens, kv_lens=kv_lens, mask=mask)
+    o = K.cross_attention(q, k, v, **kw)
+    grads = torch.autograd.grad(o, (q, k, v), do)
+    with torch.no_grad():
+        assert torch.equal(K.cross_attention(q, k, v, **kw), o)
+    keep = keep_of(q.shape[0], q.shape[1], k.shape[1], q_lens, kv_lens, mask)
+    want, tol = formula(q.detach(), k.detach(), v.detach(), do,
+                        1.0 / math.sqrt(q.shape[3]) if scale is None else scale, keep)
+    for n, x in zip(("o", "dq", "dk", "dv"), (o.detach(), *grads)):
+        assert x.dtype == q.dtype
+        within(x, want[n], tol[n], n)
+    dead_q, dead_k = ~keep.any(-1).any(1), ~keep.any(-2).any(1)
+    assert not o[dead_q].any() and not grads[0][dead_q].any()
+    assert not grads[1][dead_k].any() and not grads[2][dead_k].any()
+    return o.detach(), grads
+
+
+def inputs(dtype, b, tq, tk, h, hk, d, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed + 7919 * tq + tk)
+    return (randn(g, b, tq, h, d, dtype=dtype), randn(g, b, tk, hk, d, dtype=dtype),
+            randn(g, b, tk, hk, d, dtype=dtype), randn(g, b, tq, h, d, dtype=dtype), g)
+
+
+SIZES = [
+    # b, tq, tk, h, hk, d
+    (1, 1, 1, 1, 1, 1), (2, 1, 62, 4, 4, 64), (3, 1, 700, 8, 2, 128), (1, 1, 5000, 8, 1, 64),
+    (2, 5, 33, 6, 3, 36), (1, 33, 31, 2, 1, 5), (2, 17, 129, 2, 2, 256), (3, 62, 196, 1, 1, 256),
+    (2, 196, 32, 4, 4, 64), (1, 130, 257, 4, 2, 80), (1, 300, 1, 2, 2, 96), (2, 129, 65, 3, 1, 200),
+    (1, 7, 2100, 4, 1, 128), (1, 1025, 40, 2, 1, 128), (9, 31, 64, 16, 8, 32),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("size", SIZES, ids=["x".join(map(str, s)) for s in SIZES])
+def test_attention_sizes(dtype, size):
+    q, k, v, do, _ = inputs(dtype, *size)
+    check(q, k, v, do)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("size", [(4, 40, 70, 4, 2, 64), (4, 3, 300, 4, 1, 128),
+                                  (5, 150, 33, 2, 2, 256)],
+                         ids=["tile", "few", "wide"])
+def test_attention_lengths_and_masks(dtype, size):
+    """Empty and full lengths, lengths past the tensors (clamped), a mask that
+    empties one sample; what masked places hold does not matter."""
+    b, tq, tk = size[:3]
+    q, k, v, do, g = inputs(dtype, *size)
+    kv_lens = torch.randint(1, tk + 1, (b,), generator=g, device="cuda").int()
+    q_lens = torch.randint(1, tq + 1, (b,), generator=g, device="cuda").int()
+    kv_lens[0], kv_lens[1], q_lens[1], q_lens[2] = 0, tk, 0, tq
+    mask = torch.rand(b, tk, generator=g, device="cuda") > 0.3
+    mask[3] = False
+    o, grads = check(q, k, v, do, q_lens=q_lens, kv_lens=kv_lens, mask=mask)
+    far_k, far_q = kv_lens.clone(), q_lens.clone()
+    far_k[1], far_q[2], far_k[0] = tk + 1000, tq + 1000, -5
+    live_k = keep_of(b, tq, tk, None, kv_lens, mask).any(-2).any(1)
+    live_q = torch.arange(tq, device="cuda") < q_lens.view(b, 1)
+    bad = [torch.where(x[:, :, None, None], t, t.new_tensor(w)) for x, t, w in (
+        (live_q, q, float("nan")), (live_k, k, float("inf")), (live_k, v, float("nan")),
+        (live_q, do, float("nan")))]
+    leaves = [x.requires_grad_() for x in bad[:3]]
+    o2 = K.cross_attention(*leaves, q_lens=far_q.long(), kv_lens=far_k.long(), mask=mask)
+    # rows of samples without states still carry their upstream gradient
+    got = torch.autograd.grad(o2, leaves, bad[3])
+    assert torch.equal(o2, o)
+    for x, y in zip(got, grads):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_attention_only_one_of(dtype):
+    """Lengths or a mask alone; only the queries, only the states need grad."""
+    b, tq, tk, h, hk, d = 3, 20, 90, 4, 2, 64
+    q, k, v, do, g = inputs(dtype, b, tq, tk, h, hk, d)
+    lens = torch.tensor([90, 64, 1], device="cuda", dtype=torch.int32)
+    mask = torch.rand(b, 2 * tk, generator=g, device="cuda")[:, ::2] > 0.5     # strided
+    check(q, k, v, do, kv_lens=lens)
+    _, full = check(q, k, v, do, mask=mask)
+    check(q, k, v, do, q_lens=torch.tensor([0, 20, 7], device="cuda"))
+    check(q, k, v, do, scale=0.02)
+    for i, x in enumerate((q, k, v)):
+        t = [y.clone().requires_grad_(j == i) for j, y in enumerate((q, k, v))]
+        o = K.cross_attention(*t, mask=mask)
+        assert torch.equal(torch.autograd.grad(o, t[i], do)[0], full[i])
+
+
+def test_attention_extreme_scores():
+    """Scores far apart (one state takes all), and large equal ones."""
+    b, tq, tk, h, d = 2, 40, 200, 2, 64
+    q, k, v, do, _ = inputs(F32, b, tq, tk, h, h, d)
+    with torch.no_grad():
+        o = K.cross_attention(40 * q, 40 * k, v)
+        s = (40 * q).double().transpose(1, 2) @ (40 * k).double().permute(0, 2, 3, 1) / 8
+        # fp32 scores of up to ~6e4: within (64 + 8) 2^-24 of their magnitudes
+        top2 = s.topk(2, -1)
+        sure = (top2.values[..., 0] - top2.values[..., 1]) > 40
+        want = torch.gather(v.transpose(1, 2), 2, top2.indices[..., :1].expand(-1, -1, -1, d))
+        got = o.transpose(1, 2)
+        assert bool(sure.any())
+        assert float((got - want).abs()[sure].max()) < 1e-6
+        same = K.cross_attention(q * 0 + 30, k * 0 + 30, v)       # every score 7200
+        mean = v.double().mean(1, keepdim=True).expand_as(same)
+        # a mean of 200: (200 + 48) 2^-24 of the mean magnitude, and its rounding
+        assert float((same - mean).abs().max()) <= 300 * U32 * float(v.abs().mean(1).max())
+        # a NaN or infinity in a state that IS attended to is seen
+        k2 = k.clone()
+        k2[0, 3, 0, 0] = float("nan")
+        o2 = K.cross_attention(q, k2, v)
+        assert bool(o2[0, :, 0].isnan().all()) and bool(torch.isfinite(o2[1]).all())
+        assert bool(torch.isfinite(o2[0, :, 1]).all())
+
+
+@pytest.mark.parametrize("factor", [2.0 ** -14, 2.0 ** 10])
+def test_attention_fp16_gradient_range(factor):
+    """Upstream gradients near either end of fp16's range: dS itself would
+    leave the range, the results do not."""
+    q, k, v, do, _ = inputs(F16, 2, 60, 500, 4, 2, 64)
+    check(q, k, v, (do.clamp(-2, 2) * factor).to(F16))
+
+
+def test_attention_layouts():
+    """Heads before tokens, slices of one packed projection at an odd offset,
+    broadcast states, a gradient with zero strides, a head axis of stride 0."""
+    b, tq, tk, h, d = 2, 37, 51, 4, 24
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for dtype in (BF, F32):
+        q = randn(g, b, h, tq, d, dtype=dtype).transpose(1, 2)
+        packed = randn(g, b, tk, 2 * h * d + 1, dtype=dtype)
+        k = packed[..., 1:1 + h * d].view(b, tk, h, d)
+        v = packed[..., 1 + h * d:].view(b, tk, h, d)
+        do = randn(g, b, h, tq, d, dtype=dtype).transpose(1, 2)
+        check(q, k, v, do)
+        check(q, k, v, do[:, :1, :1].expand(b, tq, h, d))
+        check(q.transpose(1, 3).contiguous().transpose(1, 3), k, v, do)   # last axis not dense
+        one = randn(g, 1, tk, 1, d, dtype=dtype).requires_grad_()
+        wide = one.expand(b, tk, h, d)
+        o = K.cross_attention(q, wide, wide)
+        got, = torch.autograd.grad(o, one, do)
+        _, grads = check(q, wide, wide, do)
+        want = (grads[1].double() + grads[2].double()).sum((0, 2), keepdim=True)
+        mag = (grads[1].double().abs() + grads[2].double().abs()).sum((0, 2), keepdim=True)
+        # autograd's own sums: 2 b h terms, each partial sum rounded to the type
+        within(got, want, 2 * b * h * half_step(dtype) * mag + 1e-30, "broadcast")
+
+
+def test_attention_offsets_past_32_bits():
+    """States whose addresses pass 2^32 elements."""
+    st = (1 << 26) + 8
+    big = torch.empty(65 * st + 64, dtype=BF, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    dense = randn(g, 1, 65, 1, 64, dtype=BF)
+    k = big.as_strided((1, 65, 1, 64), (65 * st, st, 64, 1))
+    k.copy_(dense)
+    for tq in (1, 40):
+        q, do = randn(g, 1, tq, 2, 64, dtype=BF), randn(g, 1, tq, 2, 64, dtype=BF)
+        near = check(q, dense, dense, do)
+        t = [q.clone().requires_grad_(), k.detach().requires_grad_(), k.detach().requires_grad_()]
+        o = K.cross_attention(*t)
+        assert torch.equal(o, near[0])
+        for x, y in zip(torch.autograd.grad(o, t, do), near[1]):
+            assert torch.equal(x, y)
+
+
+def test_attention_empty():
+    q, k, v, do, _ = inputs(F32, 2, 5, 7, 2, 2, 16)
+    for t in ((q[:0], k[:0], v[:0]), (q[:, :0], k, v), (q, k[:, :0], v[:, :0])):
+        t = [x.clone().requires_grad_() for x in t]
+        o = K.cross_attention(*t)
+        assert o.shape == t[0].shape and not o.any()
+        for x, y in zip(torch.autograd.grad(o.sum(), t), t):
+            assert x.shape == y.shape and not x.any()
+
+
+def test_attention_gradient_against_differences():
+    """d/dh of sum(o do) along random directions against central differences
+    of the kernel's own fp32 forward, at two steps: the forward's error of
+    under 1e-6 a value (18 rows of 4 x 32 values: 5e-5 in the sum's norm)
+    over 2e-3 leaves 0.03, a step's square times the third derivative (of the
+    size of the slope) 1e-5 of it; slopes are of the size of 50."""
+    q, k, v, do, g = inputs(F32, 2, 9, 70, 4, 2, 32)
+    t = [x.clone().requires_grad_() for x in (q, k, v)]
+    grads = torch.autograd.grad(K.cross_attention(*t), t, do)
+    for i in range(3):
+        way = randn(g, *t[i].shape, dtype=F32)
+        slope = float((grads[i].double() * way.double()).sum())
+        size = float(grads[i].double().norm())      # the slope's standard deviation
+        for step in (2e-3, 1e-3):
+            val = []
+            for sign in (1, -1):
+                x = [y.detach() for y in t]
+                x[i] = x[i] + sign * step * way
+                with torch.no_grad():
+                    val.append((K.cross_attention(*x).double() * do.double()).sum())
+            got = float(val[0] - val[1]) / (2 * step)
+            assert abs(got - slope) < 0.03 + 1e-3 * size
+
+
+def test_attention_equal_calls_give_equal_bits():
+    for size in ((4, 100, 300, 8, 2, 64), (1, 1, 4000, 8, 2, 128), (1, 20, 3000, 2, 1, 64)):
+        q, k, v, do, _ = inputs(BF, *size)
+        runs = []
+        for _ in range(2):
+            t = [x.clone().requires_grad_() for x in (q, k, v)]
+            o = K.cross_attention(*t)
+            runs.append((o, *torch.autograd.grad(o, t, do)))
+        assert all(torch.equal(x, y) for x, y in zip(*runs))
+
+
+def norm_ref(x, w, rope, pos, eps, dy=None):
+    """y (and dx, dw) of the formulas in 64 bits, with bounds for fp32."""
+    d, x, w = x.shape[3], x.double(), w.double()
+    r = 1.0 / torch.sqrt((x * x).mean(-1, keepdim=True) + eps)
+    n = x * r
+    half = 0 if rope is None else rope.dim // 2
+    if half:
+        per = half // rope.axes
+        freq = rope.base ** (-(torch.arange(half, device="cuda") % per).double() / per)
+        p = pos.double().view(*pos.shape[:2], rope.axes)
+        ang = p.repeat_interleave(per, -1) * freq                    # [B, T, half]
+        c, s = torch.cos(ang).unsqueeze(2), torch.sin(ang).unsqueeze(2)
+
+    def turn(u, sign):
+        if not half:
+            return u
+        o = u.clone()
+        a = u[..., 0:2 * half:2] if rope.interleaved else u[..., :half]
+        b = u[..., 1:2 * half:2] if rope.interleaved else u[..., half:2 * half]
+        ya, yb = a * c - sign * b * s, b * c + sign * a * s
+        if rope.interleaved:
+            o[..., 0:2 * half:2], o[..., 1:2 * half:2] = ya, yb
+        else:
+            o[..., :half], o[..., half:2 * half] = ya, yb
+        return o
+
+    def mag(u):                                                      # |ua| + |ub| at each place
+        if not half:
+            return u.abs()
+        o = u.abs().clone()
+        a = u[..., 0:2 * half:2] if rope.interleaved else u[..., :half]
+        b = u[..., 1:2 * half:2] if rope.interleaved else u[..., half:2 * half]
+        m = a.abs() + b.abs()
+        if rope.interleaved:
+            o[..., 0:2 * half:2] = o[..., 1:2 * half:2] = m
+        else:
+            o[..., :half] = o[..., half:2 * half] = m
+        return o
+    e = (d + 24) * U32
+    y, y_tol = turn(n * w, 1), e * mag(n * w)
+    if dy is None:
+        return y, y_tol
+    du, du_mag = turn(dy.double(), -1), mag(dy.double())
+    dn, dn_mag = du * w, du_mag * w.abs()
+    mean = (dn * n).mean(-1, keepdim=True)
+    mean_mag = (dn_mag * n.abs()).mean(-1, keepdim=True)
+    dx = r * (dn - n * mean)
+    dx_tol = (2 * d + 60) * U32 * r * (dn_mag + n.abs() * mean_mag)
+    count = x.shape[0] * x.shape[1] * x.shape[2]
+    dw = (du * n).sum((0, 1, 2))
+    dw_tol = (count + d + 60) * U32 * (du_mag * n.abs()).sum((0, 1, 2))
+    return y, y_tol, dx, dx_tol, dw, dw_tol
+
+
+def check_norm(q, k, wq, wk, rope, q_pos, k_pos, out_dtype=None, eps=1e-6, g=None):
+    leaves = [x for x in (q, k, wq, wk) if x is not None]
+    for x in leaves:
+        x.requires_grad_()
+    y = K.qk_norm_rope(q, k, wq, wk, eps=eps, rope=rope, q_pos=q_pos, k_pos=k_pos,
+                       out_dtype=out_dtype)
+    with torch.no_grad():
+        again = K.qk_norm_rope(q, k, wq, wk, eps=eps, rope=rope, q_pos=q_pos, k_pos=k_pos,
+                               out_dtype=out_dtype)
+    dy = [None if x is None else randn(g, *x.shape, dtype=x.dtype) for x in y]
+    grads = torch.autograd.grad([x for x in y if x is not None], leaves,
+                                [x for x in dy if x is not None])
+    grads = dict(zip([n for n, x in (("q", q), ("k", k), ("wq", wq), ("wk", wk))
+                      if x is not None], grads))
+    for i, (name, x, w, pos) in enumerate((("q", q, wq, q_pos), ("k", k, wk, k_pos))):
+        if x is None:
+            assert y[i] is None
+            continue
+        axes = 1 if rope is None else rope.axes
+        b, t = x.shape[:2]
+        if pos is None:
+            pos = torch.arange(t, device="cuda")
+        shape = (b, t) if axes == 1 else (b, t, axes)
+        ref = norm_ref(x.detach(), w.detach(), rope, pos.expand(shape), eps, dy[i])
+        u, ui = half_step(y[i].dtype), half_step(x.dtype)
+        low = 2.0 ** -25 if F16 in (x.dtype, y[i].dtype) else 1e-37
+        assert torch.equal(again[i], y[i]) and y[i].is_contiguous()
+        within(y[i].detach(), ref[0], ref[1] + u * ref[0].abs() + low, name)
+        within(grads[name], ref[2], ref[3] + ui * ref[2].abs() + low, "d" + name)
+        within(grads["w" + name], ref[4], ref[5] + U32 * ref[4].abs() + 1e-37, "dw" + name)
+
+
+NORMS = [
+    # dtype, out, b, tq, tk, h, hk, d, rot, axes, interleaved
+    (BF, BF, 2, 1, 1, 4, 2, 64, 64, 1, False), (F16, F16, 3, 7, 5, 6, 3, 80, 80, 1, False),
+    (F32, F32, 2, 196, 62, 4, 4, 64, 64, 2, False), (F32, BF, 2, 33, 9, 4, 1, 128, 64, 1, True),
+    (F32, F16, 1, 10, 300, 2, 2, 256, 256, 1, False), (BF, BF, 2, 40, 20, 8, 2, 256, 128, 2, True),
+    (BF, BF, 1, 5, 6, 3, 1, 36, 36, 1, False), (F32, F32, 2, 5, 6, 3, 1, 36, 12, 1, True),
+    (F32, F32, 1, 3, 2, 1, 1, 2, 2, 1, True), (F16, F16, 2, 9, 9, 5, 5, 250, 200, 1, False),
+    (BF, BF, 3, 4000, 100, 2, 1, 32, 32, 1, False), (F32, F32, 2, 20, 20, 2, 2, 96, 0, 1, False),
+    (BF, BF, 1, 20, 2, 2, 2, 96, 32, 1, False), (BF, BF, 4, 3000, 11, 4, 2, 64, 64, 1, True),
+]
+
+
+@pytest.mark.parametrize("case", NORMS, ids=[str(i) for i in range(len(NORMS))])
+def test_norm_rope(case):
+    dtype, out, b, tq, tk, h, hk, d, rot, axes, inter = case
+    g = torch.Generator(device="cuda").manual_seed(d + tq)
+    rope = K.Rope(rot, axes=axes, interleaved=inter) if rot else None
+    q, k = randn(g, b, tq, h, d, dtype=dtype), 3 * randn(g, b, tk, hk, d, dtype=dtype)
+    wq, wk = randn(g, d, dtype=F32), randn(g, d, dtype=F32)
+    tail = () if axes == 1 else (axes,)
+    pos = [None, None]
+    if rope is not None and (axes > 1 or d % 64 == 0):
+        pos = [torch.randint(-50, 4000, (b, t, *tail), generator=g, device="cuda")
+               for t in (tq, tk)]
+        if d == 128:
+            pos = [p.int() for p in pos]
+    check_norm(q, k, wq, wk, rope, *pos, out_dtype=out, g=g)
+    check_norm(q.detach(), None, wq.detach(), None, rope, pos[0], None, out_dtype=out, g=g)
+
+
+def test_norm_layouts_and_rows_of_zeros():
+    """Slices of one packed projection at an odd offset, heads before tokens,
+    shared positions, an empty side, a row of zeros."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    b, t, h, d = 2, 19, 3, 16
+    rope = K.Rope(16)
+    for dtype in (BF, F32):
+        packed = randn(g, b, t, 2 * h * d + 1, dtype=dtype)
+        q = packed[..., 1:1 + h * d].view(b, t, h, d)
+        k = randn(g, b, h, t, d, dtype=dtype).transpose(1, 2)
+        k[0, 0] = 0
+        w = torch.rand(d, generator=g, device="cuda") + 0.5
+        pos = torch.arange(5, 5 + t, device="cuda")
+        check_norm(q.detach(), k.detach(), w.clone(), w.clone(), rope, pos, pos, g=g)
+        y = K.qk_norm_rope(q.detach()[:, :0], k.detach(), w, w, rope=rope)
+        assert y[0].numel() == 0 and y[1].shape == k.shape
+        one = [x.detach().clone().requires_grad_() for x in (q[:, :0], k, w, w)]
+        y = K.qk_norm_rope(*one, rope=rope)
+        grads = torch.autograd.grad((y[0].sum() + y[1].sum(),), one)
+        assert grads[0].numel() == 0 and not grads[2].any()
+
+
+def test_norm_far_positions():
+    """Positions to 2^40 and negative ones against 50-digit angles: the step
+    table is off by at most 2^-65 of a circle a position."""
+    getcontext().prec = 50
+    rope = K.Rope(16, base=10000.0)
+    pos = torch.tensor([[0, 1, -1, 1000003, (1 << 31) + 12345, -(1 << 33) - 7, (1 << 40) - 1]],
+                       device="cuda")
+    x = torch.zeros(1, 7, 1, 16, device="cuda")
+    x[..., :8] = 1.0
+    y, _ = K.qk_norm_rope(x, None, torch.ones(16, device="cuda"), None, eps=0.0, rope=rope,
+                          q_pos=pos)
+    n = math.sqrt(2.0)                                  # 1 / sqrt(8 / 16)
+    pi2 = Decimal("6.2831853071795864769252867665590057683943387987502")
+    for j, p in enumerate(pos[0].tolist()):
+        for i in range(8):
+            a = float((Decimal(p) * Decimal(10000) ** (Decimal(-i) / 8)) % pi2)
+            tol = 24 * U32 * n + abs(p) * 2.0 ** -64 * 6.3
+            assert abs(float(y[0, j, 0, i]) - n * math.cos(a)) <= tol
+            assert abs(float(y[0, j, 0, i + 8]) - n * math.sin(a)) <= tol
+
+
+def block(x, c, w, rope, grid, lens, heads_, d, dtype):
+    """Queries from regions, keys and values from words, normed and rotated,
+    then attention: the operators as they are used together."""
+    b, t, _ = x.shape
+    q = x.view(b, t, heads_, d)
+    k, v = c.view(b, -1, 2, heads_, d).unbind(2)
+    q, k = K.qk_norm_rope(q, k, *w, rope=rope, q_pos=grid,
+                          k_pos=torch.zeros(k.shape[1], 2, device="cuda", dtype=torch.int64),
+                          out_dtype=dtype)
+    return K.cross_attention(q, k, v.to(dtype), kv_lens=lens)
+
+
+def test_run_together_captured_and_on_another_stream():
+    """norm + rotation -> attention -> gradients: on a side stream, and as a
+    captured graph replayed on new inputs between eager calls, all equal to
+    the eager result bit for bit."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    b, h, d, t = 3, 4, 32, 13
+    rope, grid = K.Rope(d, axes=2), K.grid_positions(14, 14)
+
+    def make():
+        return [randn(g, b, 196, h * d, dtype=F32), randn(g, b, t, 2 * h * d, dtype=F32),
+                1 + 0.1 * randn(g, d, dtype=F32), 1 + 0.1 * randn(g, d, dtype=F32),
+                randn(g, b, 196, h, d, dtype=BF),
+                torch.randint(0, t + 1, (b,), generator=g, device="cuda").int()]
+
+    def step(x, c, wq, wk, do, lens):
+        leaves = [y.detach().requires_grad_() for y in (x, c, wq, wk)]
+        o = block(leaves[0], leaves[1], leaves[2:], rope, grid, lens, h, d, BF)
+        return [o.detach(), *torch.autograd.grad(o, leaves, do)]
+
+    data = [make() for _ in range(3)]
+    eager = [step(*x) for x in data]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step(*data[1])
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, y) for x, y in zip(other, eager[1]))
+
+    held = [x.clone() for x in data[0]]
+    with torch.cuda.stream(side):
+        step(*held)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*held)
+    for i in (0, 1, 2, 1, 0):
+        for x, y in zip(held, data[i]):
+            x.copy_(y)
+        graph.replay()
+        again = step(*data[2 - i])
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, eager[i]))
+        assert all(torch.equal(x, y) for x, y in zip(again, eager[2 - i]))
+
+
+def test_token_steps_against_whole():
+    """One token at a time against kept keys and values gives what the whole
+    sequence gives, within the two roundings."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    b, t, s, h, hk, d = 2, 6, 90, 8, 2, 64
+    q, k, v = (randn(g, b, n, m, d, dtype=BF) for n, m in ((t, h), (s, hk), (s, hk)))
+    w, rope = torch.ones(d, device="cuda"), K.Rope(d)
+    lens = torch.tensor([90, 41], device="cuda")
+    yq, yk = K.qk_norm_rope(q, k, w, w, rope=rope)
+    whole = K.cross_attention(yq, yk, v, kv_lens=lens)
+    for i in range(t):
+        pos = torch.full((b, 1), i, device="cuda")
+        qi, none = K.qk_norm_rope(q[:, i:i + 1], None, w, None, rope=rope, q_pos=pos)
+        assert none is None and torch.equal(qi, yq[:, i:i + 1])
+        one = K.cross_attention(qi, yk, v, kv_lens=lens)
+        want, tol = formula(qi, yk, v, torch.zeros_like(qi), d ** -0.5,
+                            keep_of(b, 1, s, None, lens))
+        within(one, want["o"], tol["o"], "token")
+        within(whole[:, i:i + 1], want["o"], tol["o"], "whole")

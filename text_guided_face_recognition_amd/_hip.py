@@ -137,6 +137,14 @@ SIGNATURES = {
     "tgfr_proj_dw": [P, L, P, L, I, I, I, P, L, P, P],
     "tgfr_arc_dx_ws": [I, I, I, P],
     "tgfr_arc_dx": [P, P, L, I, I, I, P, P, F, P, P, P],
+    "tgfr_cross_attention_ws": [I, I, I, I, I, I, I, I, P],
+    "tgfr_cross_attention_fwd": [P, P, P, P, P, P, P, P, L, I, I, I, I, I, I, F, I, P, P, P],
+    "tgfr_cross_attention_bwd": [P, P, P, P, P, P, P, P, P, P, P, P, L, I, I, I, I, I, I, F, I,
+                                 P, P, P],
+    "tgfr_qk_norm_rope_ws": [I, P],
+    "tgfr_qk_norm_rope_fwd": [P, P, P, P, P, P, P, P, P, I, P, I, I, I, I, F, I, I, P],
+    "tgfr_qk_norm_rope_bwd": [P, P, P, P, P, P, P, P, P, P, P, I, P, I, I, I, I, F, I, I, P, P,
+                              P, P],
 }
 
 

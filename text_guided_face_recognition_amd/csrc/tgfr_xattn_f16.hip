@@ -1,0 +1,8 @@
+// The f16 kernels of cross attention (tgfr_xattn.h).
+#include "tgfr_xattn.h"
+
+namespace tgfr {
+int xattn_run_f16(const XArgs& a, int what, void* stream) {
+  return x_by_width<XF16>(a, what, stream);
+}
+}  // namespace tgfr
