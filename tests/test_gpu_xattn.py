@@ -551,3 +551,12 @@ def test_token_steps_against_whole():
                             keep_of(b, 1, s, None, lens))
         within(one, want["o"], tol["o"], "token")
         within(whole[:, i:i + 1], want["o"], tol["o"], "whole")
+
+
+def test_second_derivatives_are_refused():
+    q, k, v, do, _ = inputs(F32, 1, 3, 4, 2, 2, 8)
+    q.requires_grad_()
+    w = torch.ones(8, device="cuda", requires_grad=True)
+    for o in (K.cross_attention(q, k, v), K.qk_norm_rope(q, None, w, None)[0]):
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            torch.autograd.grad(o.sum(), q, create_graph=True)

@@ -181,6 +181,25 @@ def _bind(handle):
     return handle
 
 
+_front = None
+
+
+def front():
+    """The compiled torch front-end (csrc/tgfr_front.cpp), bound to the entry
+    points of the loaded kernel library."""
+    global _front
+    if _front is None:
+        from importlib import machinery, util
+        handle = lib()
+        loader = machinery.ExtensionFileLoader("tgfr_front", _build.FRONT)
+        mod = util.module_from_spec(util.spec_from_loader("tgfr_front", loader))
+        loader.exec_module(mod)
+        mod.bind({n: C.cast(getattr(handle, n), P).value for n in SIGNATURES
+                  if n.startswith(("tgfr_cross_attention", "tgfr_qk_norm_rope"))})
+        _front = mod
+    return _front
+
+
 def exported_symbols():
     return [n for n in SIGNATURES if getattr(lib(), n, None) is not None]
 

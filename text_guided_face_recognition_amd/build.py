@@ -1,9 +1,12 @@
-"""Build libtgfr_hip.so (the C-ABI kernel library) in-tree for gfx950.
+"""Build libtgfr_hip.so (the C-ABI kernel library) in-tree for gfx950, and
+tgfr_front.so, the compiled torch front-end of some of its entries.
 
     python -m text_guided_face_recognition_amd.build [--verbose]
 
 Each csrc/*.hip compiles to its own object (in parallel, with per-file
-flags), then hipcc links the shared library.  Nothing here depends on torch.
+flags), then hipcc links the shared library, which does not depend on torch.
+csrc/tgfr_front.cpp (host code against torch's headers) is a Python module of
+its own beside it.
 
 The library is stamped with a hash of everything it is built from (sources,
 headers, this file's flags): ``stale()`` compares the stamp with the tree, and
@@ -14,9 +17,11 @@ from __future__ import annotations
 
 import glob
 import hashlib
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -24,6 +29,8 @@ CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 LIB = os.path.join(LIB_DIR, "libtgfr_hip.so")
+FRONT_SRC = os.path.join(CSRC, "tgfr_front.cpp")
+FRONT = os.path.join(LIB_DIR, "tgfr_front.so")
 STAMP = LIB + ".sha256"
 INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 HIPCC = "/opt/rocm/bin/hipcc"
@@ -49,16 +56,36 @@ def sources():
 
 def deps():
     """Every file the library is built from."""
-    return sorted(sources() + glob.glob(os.path.join(CSRC, "*.h")) +
+    return sorted(sources() + [FRONT_SRC] + glob.glob(os.path.join(CSRC, "*.h")) +
                   glob.glob(os.path.join(INCLUDE, "*.h")) + [os.path.abspath(__file__)])
+
+
+def torch_dir():
+    """torch's folder, found without importing it."""
+    return importlib.util.find_spec("torch").submodule_search_locations[0]
+
+
+def torch_version():
+    with open(os.path.join(torch_dir(), "version.py")) as f:
+        return f.read()
+
+
+def front_command():
+    t = torch_dir()
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1",
+            "-DUSE_ROCM=1", "-I", INCLUDE, "-isystem", os.path.join(t, "include"), "-isystem",
+            os.path.join(t, "include", "torch", "csrc", "api", "include"), "-isystem",
+            "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"], FRONT_SRC, "-o",
+            FRONT + ".tmp", "-L" + os.path.join(t, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu",
+            "-ltorch_python"]
 
 
 def source_hash(extra=()):
     """Hash of every input of the build: the sources and headers, this file,
-    the compiler, the target and any extra flags (a debug / experiment build
+    the compiler, the target, torch's version and any extra flags (a debug / experiment build
     never carries the default build's stamp)."""
     h = hashlib.sha256()
-    h.update(f"{HIPCC}|{ARCH}|{' '.join(extra)}".encode())
+    h.update(f"{HIPCC}|{ARCH}|{' '.join(extra)}|{torch_version()}".encode())
     for p in deps():
         h.update(os.path.relpath(p, os.path.dirname(PKG)).encode())
         with open(p, "rb") as f:
@@ -68,7 +95,7 @@ def source_hash(extra=()):
 
 def stale():
     """True when the library is missing or was built from other sources."""
-    if not (os.path.exists(LIB) and os.path.exists(STAMP)):
+    if not all(os.path.exists(p) for p in (LIB, FRONT, STAMP)):
         return True
     with open(STAMP) as f:
         return f.read().strip() != source_hash()
@@ -112,13 +139,17 @@ def _build_locked(verbose, extra):
         name = os.path.basename(src)
         obj = os.path.join(OBJ_DIR, name.replace(".hip", ".o"))
         jobs.append(([*common, *FILE_FLAGS.get(name, []), "-c", src, "-o", obj], obj))
+    # the files that take longest first
+    jobs.sort(key=lambda j: -os.path.getsize(j[0][-3]) - 10**6 * ("xattn_" in j[1]))
+    jobs.append((front_command(), None))
     workers = max(1, min(len(jobs), int(os.environ.get("MAX_JOBS", os.cpu_count() or 4))))
     with ThreadPoolExecutor(workers) as ex:
         list(ex.map(lambda j: _run(j[0], verbose), jobs))
     tmp = LIB + ".tmp"
     _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-fno-gpu-rdc", "-o", tmp,
-          *[o for _, o in jobs]], verbose)
+          *sorted(o for _, o in jobs if o)], verbose)
     os.replace(tmp, LIB)
+    os.replace(FRONT + ".tmp", FRONT)
     with open(STAMP, "w") as f:
         f.write(digest + "\n")
     return LIB

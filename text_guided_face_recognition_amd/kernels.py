@@ -2218,123 +2218,8 @@ def text_heading(words_emb, taps, conv_b, mode="fp32", words=None, sent=None, ro
 # ---------------------------------------------------------------------------
 # Cross attention between sequences of different lengths, and the per-head
 # norm + position rotation of its queries and keys (csrc/tgfr_xattn.h,
-# csrc/tgfr_rope.hip)
-
-_TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
-_L12, _L24, _L30 = (ctypes.c_longlong * n for n in (12, 24, 30))
-
-
-def _head_tensor(name, x):
-    if x.dim() != 4:
-        raise ValueError(f"{name} must be [batch, tokens, heads, head_dim], got {tuple(x.shape)}")
-    if x.dtype not in _TYPES:
-        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {x.dtype}")
-
-
-def _same_device(x, **others):
-    """The device checks come last, so that every other refusal needs no GPU."""
-    for name, t in others.items():
-        if t is not None and t.device != x.device:
-            raise RuntimeError(f"{name} is on {t.device}, the queries on {x.device}")
-    if not x.is_cuda:
-        raise RuntimeError("tgfr kernels take device tensors only (no CPU path)")
-
-
-class _On:
-    """Makes a tensor's device the current one for the calls inside (they
-    launch on that device's current stream)."""
-
-    def __init__(self, x):
-        self.ctx = None if x.device.index == torch.cuda.current_device() else \
-            torch.cuda.device(x.device)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
-
-
-def _ws(name, *args):
-    out = ctypes.c_longlong(0)
-    rc = getattr(_hip.lib(), name)(*args, ctypes.byref(out))
-    if rc != 0:
-        raise RuntimeError(f"{name} failed with code {rc}")
-    return out.value
-
-
-def _xattn_fwd(q, k, v, scale, q_lens, kv_lens, mask, want_lse):
-    b, tq, h, d = q.shape
-    tk, hk = k.shape[1], k.shape[2]
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(b, hk, tq * (h // hk), dtype=torch.float32, device=q.device) \
-        if want_lse else None
-    if not q.numel() or not k.numel():
-        return o.zero_(), (lse.fill_(float("inf")) if want_lse else None)
-    t = _TYPES[q.dtype]
-    with _On(q):
-        n = _ws("tgfr_cross_attention_ws", b, tq, tk, h, hk, d, t, 0)
-        ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
-        s = _L12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3])
-        call("tgfr_cross_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-             ctypes.addressof(s), ptr(q_lens), ptr(kv_lens), ptr(mask),
-             0 if mask is None else mask.stride(0), b, tq, tk, h, hk, d, scale, t, ptr(lse),
-             ptr(ws), _hip.stream())
-    return o, lse
-
-
-class CrossAttention(torch.autograd.Function):
-    """softmax(scale Q K^T) V with Q [B, Tq, H, D], K and V [B, Tk, Hk, D]
-    (tgfr_cross_attention_fwd / _bwd)."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, scale, q_lens, kv_lens, mask):
-        o, lse = _xattn_fwd(q, k, v, scale, q_lens, kv_lens, mask, True)
-        ctx.save_for_backward(q, k, v, o, lse, q_lens, kv_lens, mask)
-        ctx.scale = scale
-        return o
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, do):
-        q, k, v, o, lse, q_lens, kv_lens, mask = ctx.saved_tensors
-        b, tq, h, d = q.shape
-        tk, hk = k.shape[1], k.shape[2]
-        want_kv = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) if want_kv else None
-                  for _ in range(2))
-        if not q.numel() or not k.numel():
-            for x in (dq, dk, dv):
-                if x is not None:
-                    x.zero_()
-            return dq, dk, dv, None, None, None, None
-        do = _rows(do)
-        t = _TYPES[q.dtype]
-        with _On(q):
-            n = _ws("tgfr_cross_attention_ws", b, tq, tk, h, hk, d, t, 1)
-            ws = torch.empty(n, dtype=torch.float32, device=q.device)
-            g = (dk.stride()[:3] + dv.stride()[:3]) if want_kv else (0,) * 6
-            s = _L24(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3],
-                     *do.stride()[:3], *dq.stride()[:3], *g)
-            call("tgfr_cross_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                 o.data_ptr(), do.data_ptr(), dq.data_ptr(), ptr(dk), ptr(dv),
-                 ctypes.addressof(s), ptr(q_lens), ptr(kv_lens), ptr(mask),
-                 0 if mask is None else mask.stride(0), b, tq, tk, h, hk, d, ctx.scale, t,
-                 lse.data_ptr(), ws.data_ptr(), _hip.stream())
-        return dq, dk, dv, None, None, None, None
-
-
-def _lens_tensor(name, lens, n):
-    if lens is None:
-        return None
-    if not torch.is_tensor(lens) or lens.dtype not in (torch.int32, torch.int64) or \
-            tuple(lens.shape) != (n,):
-        raise ValueError(f"{name} must be an int32 or int64 tensor of {n} lengths")
-    return lens
-
+# csrc/tgfr_rope.hip; checks, allocation and autograd nodes in
+# csrc/tgfr_front.cpp)
 
 def cross_attention(q, k, v, scale=None, q_lens=None, kv_lens=None, mask=None):
     """Attention of q [B, Tq, H, D] to the states k, v [B, Tk, Hk, D] of
@@ -2345,49 +2230,17 @@ def cross_attention(q, k, v, scale=None, q_lens=None, kv_lens=None, mask=None):
     H is a multiple of Hk: query head h reads key head h // (H // Hk).  All
     three have one type (float32, bfloat16, float16); D <= 256, any strides
     (a last axis that is not dense is copied).  scale: 1 / sqrt(D) by default.
-    q_lens, kv_lens [B] (device): tokens of each sample; rows past q_lens are
-    zero and get no gradient, states past kv_lens are not read.  mask [B, Tk]
-    (bool, device): False leaves a state out.  A row without any state gives
-    zero.  One token (Tq = 1) splits the states over the whole card.
+    q_lens, kv_lens [B] (int32 or int64, device): tokens of each sample; rows
+    past q_lens are zero and get no gradient, states past kv_lens are not
+    read.  mask [B, Tk] (bool, device): False leaves a state out.  A row
+    without any state gives zero.  One token (Tq = 1) splits the states over
+    the whole card.
 
     Sums, softmax statistics and accumulators are fp32; bf16 / fp16 round the
     probabilities (backward: dS) to the type as matrix operands.  Equal calls
-    give equal bits.  Only enqueues work on the current stream: can be
-    captured into a HIP graph."""
-    for name, x in (("q", q), ("k", k), ("v", v)):
-        _head_tensor(name, x)
-    b, tq, h, d = q.shape
-    if k.shape != v.shape:
-        raise ValueError(f"k and v differ: {tuple(k.shape)}, {tuple(v.shape)}")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"q, k and v need one type, got {q.dtype}, {k.dtype}, {v.dtype}")
-    tk, hk = k.shape[1], k.shape[2]
-    if k.shape[0] != b or k.shape[3] != d:
-        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} need one batch and head size")
-    if not 1 <= d <= 256:
-        raise ValueError(f"head size must be 1 to 256, got {d}")
-    if hk < 1 or h < 1 or h % hk:
-        raise ValueError(f"{h} query heads are no multiple of {hk} key heads")
-    if max(tq * h, tk * hk) * b > 1 << 30:
-        raise ValueError("at most 2^30 rows of queries or keys")
-    scale = 1.0 / d ** 0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"scale must be positive and finite, got {scale}")
-    q_lens = _lens_tensor("q_lens", q_lens, b)
-    kv_lens = _lens_tensor("kv_lens", kv_lens, b)
-    if mask is not None and (mask.dtype != torch.bool or tuple(mask.shape) != (b, tk)):
-        raise ValueError(f"mask must be a bool tensor [{b}, {tk}]")
-    _same_device(q, k=k, v=v, q_lens=q_lens, kv_lens=kv_lens, mask=mask)
-    if q_lens is not None:
-        q_lens = q_lens.to(torch.int32).contiguous()
-    if kv_lens is not None:
-        kv_lens = kv_lens.to(torch.int32).contiguous()
-    if mask is not None:
-        mask = _rows(mask)
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return CrossAttention.apply(q, k, v, scale, q_lens, kv_lens, mask)
-    return _xattn_fwd(q, k, v, scale, q_lens, kv_lens, mask, False)[0]
+    give equal bits.  Only enqueues work on the current stream of q's device:
+    can be captured into a HIP graph.  Second derivatives are refused."""
+    return _hip.front().cross_attention(q, k, v, scale, q_lens, kv_lens, mask)
 
 
 class Rope:
@@ -2425,93 +2278,6 @@ def grid_positions(h, w, device="cuda"):
     return torch.stack([i // w, i % w], 1)
 
 
-def _positions(name, pos, rope, b, t):
-    """(positions or None, their strides over samples, tokens, axes)."""
-    axes = 1 if rope is None else rope.axes
-    if pos is None:
-        if axes > 1:
-            raise ValueError(f"{axes} position axes need {name}")
-        return None, (0, 0, 0)
-    if rope is None:
-        raise ValueError(f"{name} without a rope")
-    if pos.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"{name} must be int32 or int64, got {pos.dtype}")
-    tail = (t,) if axes == 1 else (t, axes)
-    if tuple(pos.shape) == tail:
-        s = (0, *pos.stride())
-    elif tuple(pos.shape) == (b, *tail):
-        s = pos.stride()
-    else:
-        raise ValueError(f"{name} must be {list(tail)} or {[b, *tail]}, got {list(pos.shape)}")
-    return pos, (s if axes > 1 else (*s, 0))
-
-
-def _norm_shapes(q, k, gq, gk, yq, yk, sq, sk):
-    out = []
-    for x, g, y, s in ((q, gq, yq, sq), (k, gk, yk, sk)):
-        if x is None:
-            out += [0] * 15
-        else:
-            b, t, h, _ = x.shape
-            out += [b, t, h, *x.stride()[:3], *((0, 0, 0) if g is None else g.stride()[:3]),
-                    *y.stride()[:3], *s]
-    return _L30(*out)
-
-
-def _norm_call(name, q, k, g, y, wq, wk, qp, kp, cfg, tail):
-    eps, rope, sq, sk, out_dtype = cfg
-    x = q if q is not None else k
-    shapes = _norm_shapes(q, k, *(g or (None, None)), *y, sq, sk)
-    pos = qp if qp is not None else kp
-    with _On(x):
-        call(name, ptr(q), ptr(k), *((ptr(g[0]), ptr(g[1])) if g else ()), ptr(y[0]), ptr(y[1]),
-             ctypes.addressof(shapes), ptr(wq), ptr(wk), ptr(qp), ptr(kp),
-             int(pos is not None and pos.dtype == torch.int32),
-             None if rope is None else rope.turn.data_ptr(), 0 if rope is None else rope.dim,
-             1 if rope is None else rope.axes, int(rope is not None and rope.interleaved),
-             x.shape[3], eps, _TYPES[x.dtype], _TYPES[out_dtype], *tail, _hip.stream())
-
-
-def _norm_fwd(q, k, wq, wk, qp, kp, cfg):
-    y = [None if x is None else torch.empty(x.shape, dtype=cfg[-1], device=x.device)
-         for x in (q, k)]
-    _norm_call("tgfr_qk_norm_rope_fwd", q, k, None, y, wq, wk, qp, kp, cfg, ())
-    return y
-
-
-class QKNormRope(torch.autograd.Function):
-    """Per-head RMS norm and rotation of q and k (tgfr_qk_norm_rope_fwd /
-    _bwd)."""
-
-    @staticmethod
-    def forward(ctx, q, k, wq, wk, qp, kp, cfg):
-        yq, yk = _norm_fwd(q, k, wq, wk, qp, kp, cfg)
-        ctx.save_for_backward(q, k, wq, wk, qp, kp)
-        ctx.cfg = cfg
-        return yq, yk
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gq, gk):
-        q, k, wq, wk, qp, kp = ctx.saved_tensors
-        g = [None if x is None else
-             (torch.zeros(x.shape, dtype=ctx.cfg[-1], device=x.device) if d is None else _rows(d))
-             for x, d in ((q, gq), (k, gk))]
-        dx = [None if x is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-              for x in (q, k)]
-        x = q if q is not None else k
-        d = x.shape[3]
-        need = [w is not None and ctx.needs_input_grad[2 + i] for i, w in enumerate((wq, wk))]
-        dw = [torch.empty(d, dtype=torch.float32, device=x.device) if n else None for n in need]
-        ws = None
-        if any(need):
-            ws = torch.empty(_ws("tgfr_qk_norm_rope_ws", d), dtype=torch.float32,
-                             device=x.device)
-        _norm_call("tgfr_qk_norm_rope_bwd", q, k, g, dx, wq, wk, qp, kp, ctx.cfg,
-                   (ptr(ws), ptr(dw[0]), ptr(dw[1])))
-        return dx[0], dx[1], dw[0], dw[1], None, None, None
-
-
 def qk_norm_rope(q, k, q_weight, k_weight, eps=1e-6, rope=None, q_pos=None, k_pos=None,
                  out_dtype=None):
     """RMS norm of each head of q [B, Tq, H, D] and k [B, Tk, Hk, D] (batches,
@@ -2524,44 +2290,10 @@ def qk_norm_rope(q, k, q_weight, k_weight, eps=1e-6, rope=None, q_pos=None, k_po
     and rounded once, to the same type or, from float32, to `out_dtype`.
     Positions: int32 or int64, any size, [T] or [B, T] (with more rope axes
     [T, axes] or [B, T, axes]); None: 0 .. T - 1.  D even, at most 256.  Equal
-    calls give equal bits, and the call can be captured into a HIP graph."""
-    if q is None and k is None:
-        raise ValueError("neither q nor k")
-    x = q if q is not None else k
-    for name, t, wname, w in (("q", q, "q_weight", q_weight), ("k", k, "k_weight", k_weight)):
-        if t is None:
-            continue
-        _head_tensor(name, t)
-        if t.dtype != x.dtype or t.shape[3] != x.shape[3]:
-            raise ValueError("q and k need one type and head size")
-        if w is None or w.dtype != torch.float32 or tuple(w.shape) != (t.shape[3],):
-            raise ValueError(f"{wname} must be float32 [{t.shape[3]}]")
-    d = x.shape[3]
-    if d % 2 or not 2 <= d <= 256:
-        raise ValueError(f"head size must be even and 2 to 256, got {d}")
-    if rope is not None and rope.dim > d:
-        raise ValueError(f"the rotation covers {rope.dim} of {d} elements")
-    if not eps >= 0.0:
-        raise ValueError(f"eps must not be negative, got {eps}")
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    if out_dtype != x.dtype and (x.dtype != torch.float32 or out_dtype not in _TYPES):
-        raise TypeError(f"{x.dtype} cannot be written as {out_dtype}")
-    qp = kp = None
-    sq = sk = (0, 0, 0)
-    if q is not None:
-        qp, sq = _positions("q_pos", q_pos, rope, q.shape[0], q.shape[1])
-    if k is not None:
-        kp, sk = _positions("k_pos", k_pos, rope, k.shape[0], k.shape[1])
-    if qp is not None and kp is not None and qp.dtype != kp.dtype:
-        raise TypeError(f"q_pos and k_pos need one type, got {qp.dtype}, {kp.dtype}")
-    _same_device(x, k=k, q_weight=None if q is None else q_weight,
-                 k_weight=None if k is None else k_weight, q_pos=qp, k_pos=kp,
-                 rope=None if rope is None else rope.turn)
-    q, k = (None if t is None else _rows(t) for t in (q, k))
-    wq = None if q is None else q_weight.contiguous()
-    wk = None if k is None else k_weight.contiguous()
-    cfg = (float(eps), rope, sq, sk, out_dtype)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (q, k, wq, wk)):
-        return QKNormRope.apply(q, k, wq, wk, qp, kp, cfg)
-    return tuple(_norm_fwd(q, k, wq, wk, qp, kp, cfg))
+    calls give equal bits, and the call can be captured into a HIP graph.
+    Second derivatives are refused."""
+    if rope is None:
+        return _hip.front().qk_norm_rope(q, k, q_weight, k_weight, eps, None, 0, 1, False, q_pos,
+                                         k_pos, out_dtype)
+    return _hip.front().qk_norm_rope(q, k, q_weight, k_weight, eps, rope.turn, rope.dim, rope.axes,
+                                     rope.interleaved, q_pos, k_pos, out_dtype)
