@@ -85,6 +85,13 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor dense(const Tensor& t) {
   return !t.defined() || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
 }
+// the kernels reach the rows of a tile by 32-bit offsets: tensors whose tokens
+// (or shared heads) lie further apart are copied
+Tensor near(const Tensor& t, int64_t heads) {
+  const Tensor d = dense(t);
+  const int64_t size = (int64_t)d.element_size();
+  return (160 * d.stride(1) + heads * d.stride(2) + 256) * size < (1LL << 31) ? d : d.contiguous();
+}
 Tensor floats(int64_t n, const Tensor& like) {
   return at::empty({n}, like.options().dtype(at::kFloat).requires_grad(false));
 }
@@ -177,7 +184,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
       if (want_kv) dk.zero_(), dv.zero_();
       return {dq, dk, dv, Tensor()};
     }
-    const Tensor g = dense(grads[0]);
+    const Tensor g = near(grads[0], a.h / a.hk);
     long long n = 0, st[24] = {};
     done("tgfr_cross_attention_ws",
          c_attn_ws(a.b, a.tq, a.tk, a.h, a.hk, a.d, a.type, 1, &n));
@@ -244,7 +251,7 @@ py::object cross_attention(py::handle hq, py::handle hk, py::handle hv, py::hand
   if (a.mask.defined()) a.mask = dense(a.mask);
   const bool grad = at::GradMode::is_enabled() &&
                     (a.q.requires_grad() || a.k.requires_grad() || a.v.requires_grad());
-  a.q = dense(a.q), a.k = dense(a.k), a.v = dense(a.v);
+  a.q = near(a.q, a.h / a.hk), a.k = near(a.k, 1), a.v = near(a.v, 1);
   return wrapped(grad ? CrossAttention::apply(a.q, a.k, a.v, (const Attn*)&a)
                       : attn_forward(a, nullptr));
 }

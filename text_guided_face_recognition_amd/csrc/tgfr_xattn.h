@@ -54,6 +54,7 @@ struct XArgs {
   float* part_ml;        // forward: [split][B Hk][R][2] maximum and sum
   int B, Tq, Tk, H, Hk, G, D, R;   // R = Tq G
   int splits, tiles;
+  int fast_k, fast_q;              // rows may be read as whole aligned chunks, tile by tile
   float scale;
 };
 
@@ -157,30 +158,17 @@ struct Img {
     return lds_ld16(base + r0 * ROWB + r * ROWB + (((2 * j + (lane >> 5)) ^ f(r)) << 4));
   }
   // A operand, column 32 db + lane % 32 at the rows r0 + acc_row order of
-  // B operand c (r0 a multiple of 32)
+  // B operand c (r0 a multiple of 32); 16-bit types
   static __device__ __forceinline__ uint4 tr(uint32_t base, int r0, int c, int db, int lane) {
-    if constexpr (T::ES == 2) {
-      const int i = lane & 15, g = lane >> 4, h = g >> 1, q = i >> 2;
-      const int ch = 4 * db + 2 * (g & 1) + ((i >> 1) & 1), in = 8 * (i & 1);
-      s16x4 v[2];
+    const int i = lane & 15, g = lane >> 4, h = g >> 1, q = i >> 2;
+    const int ch = 4 * db + 2 * (g & 1) + ((i >> 1) & 1), in = 8 * (i & 1);
+    s16x4 v[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = 8 * e + 4 * h + q;          // + 16 c + r0: f is the same
-        v[e] = lds_tr4(base + (r0 + 16 * c) * ROWB + r * ROWB + ((ch ^ f(r)) << 4) + in);
-      }
-      return __builtin_bit_cast(uint4, join_tr(v[0], v[1]));
-    } else {
-      const int col = 32 * db + (lane & 31), h = lane >> 5;
-      uint4 v;
-      uint32_t* o = (uint32_t*)&v;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 8 * (c & 1) + 4 * h + e;
-        o[e] = __float_as_uint(lds_ldf(base + (r0 + 16 * (c >> 1)) * ROWB + r * ROWB +
-                                       (((col >> 2) ^ f(r)) << 4) + 4 * (col & 3)));
-      }
-      return v;
+    for (int e = 0; e < 2; ++e) {
+      const int r = 8 * e + 4 * h + q;            // + 16 c + r0: f is the same
+      v[e] = lds_tr4(base + (r0 + 16 * c) * ROWB + r * ROWB + ((ch ^ f(r)) << 4) + in);
     }
+    return __builtin_bit_cast(uint4, join_tr(v[0], v[1]));
   }
   // B operand c of 32 accumulator rows
   static __device__ __forceinline__ uint4 pack(const f32x16& s, int c) {
@@ -193,40 +181,127 @@ struct Img {
   }
 };
 
-// A tile of ROWS rows in flight from global memory to LDS, held in registers.
+// A buffer over a tile: its rows lie within 2^31 bytes of its first (the entries
+// check the strides), and a lane offset of NONE reads zeros.
+constexpr uint32_t NONE = 0x80000000u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* p) {
+  return uniform_rsrc(p, NONE);
+}
+__device__ __forceinline__ uint4 buf16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+}
+__device__ __forceinline__ uint32_t buf4(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+}
+
+// A tile of ROWS rows (16-bit types) in flight from global memory to LDS, held
+// in registers.  A thread's chunks lie at fixed offsets from the tile's first
+// row, so a whole tile costs no address arithmetic but the scalar base's.
 template <class T, int DP, int ROWS, int NT>
 struct Stage {
   using I = Img<T, DP>;
-  static constexpr int N = ROWS * I::CPR / NT;
-  static_assert(ROWS * I::CPR % NT == 0, "whole chunks per thread");
+  static constexpr int N = ROWS * I::CPR / NT, STEP = NT / I::CPR;
+  static_assert(ROWS * I::CPR % NT == 0 && NT % I::CPR == 0, "whole rows per step");
   uint4 r[N];
+  uint32_t off[N];
 
-  // row(i): pointer to row i of the tile, or NULL for zeros
+  // at(i): byte offset of row i from the tile's first
+  template <class At>
+  __device__ __forceinline__ void init(At at, int D) {
+    const int ch = threadIdx.x % I::CPR;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      off[n] = ch * I::E < D ? at(threadIdx.x / I::CPR + STEP * n) + 16 * ch : NONE;
+  }
+  // the tile whose first row is at p, `rows` of them (at least 1)
+  __device__ __forceinline__ void load(const void* p, int rows) {
+    const __amdgpu_buffer_rsrc_t b = tile_rsrc(p);
+    if (rows >= ROWS) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) r[n] = buf16(b, off[n]);
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        r[n] = buf16(b, (int)threadIdx.x / I::CPR + STEP * n < rows ? off[n] : NONE);
+    }
+  }
+  // rows at any alignment and of any length: row(i) points to row i of the
+  // tile, or is NULL for zeros
   template <class Row>
-  __device__ __forceinline__ void load(Row row, int D) {
+  __device__ __forceinline__ void load_any(Row row, int D) {
+    const int ch = threadIdx.x % I::CPR;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int idx = threadIdx.x + NT * n;
-      const typename T::elem* p = row(idx / I::CPR);
-      const int ch = idx % I::CPR;
+      const typename T::elem* p = row(threadIdx.x / I::CPR + STEP * n);
       r[n] = p && ch * I::E < D ? ld_chunk<T>(p, ch, D) : zero16();
     }
   }
   __device__ __forceinline__ void store(uint32_t base) const {
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int idx = threadIdx.x + NT * n;
-      lds_st16(base + I::at(idx / I::CPR, idx % I::CPR), r[n]);
-    }
+    for (int n = 0; n < N; ++n)
+      lds_st16(base + I::at(threadIdx.x / I::CPR + STEP * n, threadIdx.x % I::CPR), r[n]);
   }
+  // zeros where keep has no bit
   template <int W>
   __device__ __forceinline__ void store_kept(uint32_t base, const uint64_t (&keep)[W]) const {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int idx = threadIdx.x + NT * n, row = idx / I::CPR;
+      const int row = threadIdx.x / I::CPR + STEP * n;
       const bool k = (keep[W == 1 ? 0 : row >> 6] >> (row & 63)) & 1;
-      lds_st16(base + I::at(row, idx % I::CPR), k ? r[n] : zero16());
+      lds_st16(base + I::at(row, threadIdx.x % I::CPR), k ? r[n] : zero16());
     }
+  }
+};
+
+// Where a kernel's A operands of 32 streamed rows come from.  16-bit types:
+// from their tile in LDS.
+template <class T, int DP>
+struct LdsSrc {
+  using I = Img<T, DP>;
+  uint32_t base;
+  int lane;
+  __device__ __forceinline__ uint4 rm(int j) const { return I::rm(base, 0, j, lane); }
+  __device__ __forceinline__ uint4 tr(int c, int db) const {
+    return I::tr(base, 0, c, db, lane);
+  }
+};
+// fp32: straight from global memory.  Its matrix instructions take 16 times as
+// long per byte as bf16's, so cache and load latency hide behind them without
+// a tile in LDS, without barriers, and with no registers for tiles in flight.
+template <int DP>
+struct MemSrc {
+  __amdgpu_buffer_rsrc_t b;
+  uint32_t row, tro[16];
+  int lane, D;
+  // the 32 rows whose first is at p; at(i): byte offset of row i; bit i of
+  // `live`: row i exists (others are zeros)
+  template <class At>
+  __device__ __forceinline__ void begin(const void* p, At at, uint32_t live, int lane_, int D_) {
+    lane = lane_;
+    D = D_;
+    b = tile_rsrc(p);
+    const int r = lane & 31, h = lane >> 5;
+    row = (live >> r) & 1 ? at(r) : NONE;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int q = acc_row(i, h);
+      tro[i] = (live >> q) & 1 ? at(q) + 4 * r : NONE;
+    }
+  }
+  __device__ __forceinline__ uint4 rm(int j) const {
+    const int d0 = 8 * j + 4 * (lane >> 5);
+    if ((D & 3) == 0) return buf16(b, d0 < D ? row + 4 * d0 : NONE);
+    return make_uint4(buf4(b, d0 < D ? row + 4 * d0 : NONE),
+                      buf4(b, d0 + 1 < D ? row + 4 * d0 + 4 : NONE),
+                      buf4(b, d0 + 2 < D ? row + 4 * d0 + 8 : NONE),
+                      buf4(b, d0 + 3 < D ? row + 4 * d0 + 12 : NONE));
+  }
+  __device__ __forceinline__ uint4 tr(int c, int db) const {
+    const bool in = 32 * db + (lane & 31) < D;
+    uint32_t v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = buf4(b, in ? tro[4 * c + e] + 128 * db : NONE);
+    return make_uint4(v[0], v[1], v[2], v[3]);
   }
 };
 
@@ -274,12 +349,18 @@ struct Keep {
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       const int j = k0 + 64 * w + lane;
-      m[w] = j < len ? (mask ? mask[j] : 1) : 0;
+      m[w] = 64 * w + lane < KT && j < len ? (mask ? mask[j] : 1) : 0;
     }
   }
-  __device__ __forceinline__ void bits(uint64_t (&keep)[W]) const {
+  // true: the whole tile
+  __device__ __forceinline__ bool bits(uint64_t (&keep)[W]) const {
+    bool all = true;
 #pragma unroll
-    for (int w = 0; w < W; ++w) keep[w] = __ballot(m[w] != 0);
+    for (int w = 0; w < W; ++w) {
+      keep[w] = __ballot(m[w] != 0);
+      all = all && keep[w] == (KT < 64 ? (1ull << (KT % 64)) - 1 : ~0ull);
+    }
+    return all;
   }
 };
 
@@ -364,20 +445,107 @@ constexpr int x_store_bytes() {
 }
 constexpr int x_max(int a, int b) { return a > b ? a : b; }
 
-// ------------------------------------------------------------------ forward ---
-// WR waves along the rows (32 each) x WS waves along the states of a tile.
+// ------------------------------------------------------------ the key stream ---
+// The states of a split, KT at a time, as the forward and dQ read them: WR
+// waves along the rows (32 each) x WS waves along the states of a tile, SUB
+// pieces of 32 states per wave and tile.
 template <class T, int DP, int WR, int WS, int KT>
-struct FwdCfg {
-  static constexpr int NT = 64 * WR * WS;
-  static constexpr int SUB = KT / WS / 32;      // 32-state pieces of a wave per tile
-  static constexpr int ML = x_max(2 * Img<T, DP>::bytes(KT), x_store_bytes<T, DP, WR, WS>());
-  static constexpr int LDS = ML + (WS > 1 ? 2 * 4 * 32 * WR * WS : 0);
+struct KeyStream {
+  using I = Img<T, DP>;
+  using E = typename T::elem;
+  static constexpr int NT = 64 * WR * WS, SUB = KT / WS / 32;
+  static constexpr bool MEM = T::ES == 4;
+  static constexpr int TILES = MEM ? 0 : 2 * I::bytes(KT);
+  static constexpr int ML = x_max(TILES, x_store_bytes<T, DP, WR, WS>());
+  // behind the tiles: 2 floats per row and wave
+  static constexpr int LDS = ML + 2 * 4 * 32 * WR * WS;
+  static constexpr int LDS32 = x_max(TILES, x_store_bytes<XF32, DP, WR, WS>()) +
+                               2 * 4 * 32 * WR * WS;
+
+  // f(piece u, its kept bits, K source, V source) for every piece of 32 states
+  // that this wave handles; all waves of the block take part.  post(): after
+  // the tile's pieces.
+  template <class F>
+  static __device__ __forceinline__ void run(const XArgs& a, const XWork& w, int klo, int khi,
+                                             int ws, F f) {
+    const int lane = threadIdx.x % 64;
+    const uint8_t* mask = a.mask ? a.mask + w.b * a.mask_sb : nullptr;
+    const E* K = x_key<E>(a.k, w.b, w.g, 0);
+    const E* V = x_key<E>(a.v, w.b, w.g, 0);
+    const uint32_t kst = (uint32_t)a.k.st * T::ES, vst = (uint32_t)a.v.st * T::ES;
+    if constexpr (MEM) {
+      static_assert(SUB == 1, "one piece per wave");
+      for (int k0 = klo + 32 * ws; k0 < khi; k0 += KT) {
+        const int j = k0 + (lane & 31);
+        const uint32_t kb = (uint32_t)__ballot(j < khi && (!mask || mask[j]));
+        MemSrc<DP> ks, vs;
+        ks.begin(K + k0 * a.k.st, [&](int r) { return r * kst; }, kb, lane, a.D);
+        vs.begin(V + k0 * a.v.st, [&](int r) { return r * vst; }, kb, lane, a.D);
+        const MemSrc<DP>*kp[1] = {&ks}, *vp[1] = {&vs};
+        const uint32_t kbs[1] = {kb};
+        f(kbs, kp, vp);
+      }
+    } else {
+      constexpr uint32_t LK = 0, LV = I::bytes(KT);
+      Stage<T, DP, KT, NT> sk, sv;
+      Keep<KT> kp;
+      sk.init([&](int r) { return r * kst; }, a.D);
+      sv.init([&](int r) { return r * vst; }, a.D);
+      auto fetch = [&](int k0) {
+        kp.load(mask, k0, khi, lane);
+        if (a.fast_k) {
+          sk.load(K + k0 * a.k.st, khi - k0);
+          sv.load(V + k0 * a.v.st, khi - k0);
+        } else {
+          sk.load_any([&](int r) { return k0 + r < khi ? K + (k0 + r) * a.k.st : nullptr; }, a.D);
+          sv.load_any([&](int r) { return k0 + r < khi ? V + (k0 + r) * a.v.st : nullptr; }, a.D);
+        }
+      };
+      if (klo < khi) fetch(klo);
+      for (int k0 = klo; k0 < khi; k0 += KT) {
+        uint64_t keep[Keep<KT>::W];
+        const bool all = kp.bits(keep);
+        __syncthreads();
+        if (all) {
+          sk.store(LK);
+          sv.store(LV);
+        } else {
+          sk.store_kept(LK, keep);
+          sv.store_kept(LV, keep);
+        }
+        __syncthreads();
+        if (k0 + KT < khi) fetch(k0 + KT);
+        uint32_t kbs[SUB];
+        LdsSrc<T, DP> ks[SUB], vs[SUB];
+        const LdsSrc<T, DP>*kq[SUB], *vq[SUB];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+          const int r0 = (ws * SUB + u) * 32;
+          kbs[u] = (uint32_t)(keep[r0 >> 6] >> (r0 & 63));
+          ks[u] = {LK + I::bytes(r0), lane};
+          vs[u] = {LV + I::bytes(r0), lane};
+          kq[u] = &ks[u];
+          vq[u] = &vs[u];
+        }
+        f(kbs, kq, vq);
+      }
+    }
+  }
 };
 
+// scores of masked states
+__device__ __forceinline__ void x_mask(f32x16& s, uint32_t kb, int h) {
+  if (kb != 0xffffffffu) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = (kb >> acc_row(e, h)) & 1 ? s[e] : -INFINITY;
+  }
+}
+
+// ------------------------------------------------------------------ forward ---
 template <class T, int DP, int WR, int WS, int KT, int OCC>
 __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_fwd(const XArgs a) {
   using I = Img<T, DP>;
-  using C = FwdCfg<T, DP, WR, WS, KT>;
+  using S = KeyStream<T, DP, WR, WS, KT>;
   using E = typename T::elem;
   const XWork w = x_work(a);
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wr = wave % WR, ws = wave / WR;
@@ -387,8 +555,6 @@ __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_fwd(const XArgs a) {
   const int len = row0 < rows ? x_len(a.kv_lens, w.b, a.Tk) : 0;
   int klo, khi;
   x_share(len, KT, a.splits, w.split, klo, khi);
-  const uint8_t* mask = a.mask ? a.mask + w.b * a.mask_sb : nullptr;
-  const uint32_t LK = 0, LV = I::bytes(KT);
   const float c2 = a.scale * LOG2E_X;
 
   uint4 qf[I::NC];
@@ -399,53 +565,36 @@ __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_fwd(const XArgs a) {
       qf[j] = p && (2 * j + h) * I::E < a.D ? ld_chunk<T>(p, 2 * j + h, a.D) : zero16();
   }
   f32x16 acc[DP / 32] = {};
+  // the reference that exponents are taken against, in the log2 domain:
+  // exp(scale s - max) = 2^(c2 s - m).  It follows the running maximum only
+  // once that has grown by 8: sums and accumulators, relative to it, stay
+  // exact, probabilities stay below 2^8, and most tiles rescale nothing.
   float m = -INFINITY, l = 0.f;
 
-  Stage<T, DP, KT, C::NT> sk, sv;
-  Keep<KT> kp;
-  auto fetch = [&](int k0) {
-    kp.load(mask, k0, khi, lane);
-    sk.load([&](int r) { return k0 + r < khi ? x_key<E>(a.k, w.b, w.g, k0 + r) : nullptr; }, a.D);
-    sv.load([&](int r) { return k0 + r < khi ? x_key<E>(a.v, w.b, w.g, k0 + r) : nullptr; }, a.D);
-  };
-  if (klo < khi) fetch(klo);
-  for (int k0 = klo; k0 < khi; k0 += KT) {
-    uint64_t keep[Keep<KT>::W];
-    kp.bits(keep);
-    __syncthreads();
-    sk.store_kept(LK, keep);
-    sv.store_kept(LV, keep);
-    __syncthreads();
-    if (k0 + KT < khi) fetch(k0 + KT);
-
-    f32x16 s[C::SUB];
+  S::run(a, w, klo, khi, ws, [&](const uint32_t (&kb)[S::SUB], auto& ks, auto& vs) {
+    f32x16 s[S::SUB];
     float top = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < C::SUB; ++u) {
-      const int r0 = (ws * C::SUB + u) * 32;
+    for (int u = 0; u < S::SUB; ++u) {
       s[u] = f32x16{};
 #pragma unroll
-      for (int j = 0; j < I::NC; ++j) s[u] = T::mma(I::rm(LK, r0, j, lane), qf[j], s[u]);
-      const uint32_t kb = (uint32_t)(keep[r0 >> 6] >> (r0 & 63));
-      if (kb != 0xffffffffu) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          s[u][e] = (kb >> acc_row(e, h)) & 1 ? s[u][e] : -INFINITY;
-      }
+      for (int j = 0; j < I::NC; ++j) s[u] = T::mma(ks[u]->rm(j), qf[j], s[u]);
+      x_mask(s[u], kb[u], h);
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
     }
-    // log2 domain: exp(scale s - max) = 2^(c2 s - m)
-    const float mn = fmaxf(m, xhalf_max(top) * c2);
-    const float mu = mn == -INFINITY ? 0.f : mn;      // no kept state so far
-    const float al = __builtin_amdgcn_exp2f(m - mu);
-    m = mn;
-    l *= al;
+    top = xhalf_max(top) * c2;
+    if (__any(top > m + 8.f || m == -INFINITY)) {
+      const float mn = fmaxf(m, top);
+      const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= al;
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db) acc[db] *= al;
+      for (int db = 0; db < DP / 32; ++db) acc[db] *= al;
+    }
+    const float mu = m == -INFINITY ? 0.f : m;        // no kept state so far
 #pragma unroll
-    for (int u = 0; u < C::SUB; ++u) {
-      const int r0 = (ws * C::SUB + u) * 32;
+    for (int u = 0; u < S::SUB; ++u) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         s[u][e] = __builtin_amdgcn_exp2f(fmaf(s[u][e], c2, -mu));
@@ -455,16 +604,15 @@ __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_fwd(const XArgs a) {
       for (int c = 0; c < I::NPF; ++c) {
         const uint4 p = I::pack(s[u], c);
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
-          acc[db] = T::mma(I::tr(LV, r0, c, db, lane), p, acc[db]);
+        for (int db = 0; db < DP / 32; ++db) acc[db] = T::mma(vs[u]->tr(c, db), p, acc[db]);
       }
     }
-  }
+  });
   l = xhalf_sum(l);
 
   float mul = 1.f;
-  if constexpr (WS > 1) {       // the waves that share rows agree on the maximum
-    const uint32_t ML = C::ML;
+  if constexpr (WS > 1) {       // the waves that share rows agree on the reference
+    constexpr uint32_t ML = 0;
     __syncthreads();
     if (h == 0) {
       lds_stf(ML + 4 * ((ws * WR + wr) * 32 + lr), m);
@@ -481,7 +629,7 @@ __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_fwd(const XArgs a) {
     m = mm;
     l = ll;
   }
-  const bool none = !(row < rows) || m == -INFINITY && l == 0.f;
+  const bool none = !(row < rows) || (m == -INFINITY && l == 0.f);
   const long long at = (long long)w.bh * a.R;
   if (a.splits == 1) {
     if (a.lse && ws == 0 && h == 0 && row < a.R)
@@ -542,12 +690,39 @@ __device__ __forceinline__ float x_down(float amax) {
   return 1.f;
 }
 
+// B operands of 32 rows (one per lane): held in registers, or, where two of
+// them would fill the registers (fp32, 256 columns), read at each use.
+template <class T, int DP>
+struct Rows32 {
+  using I = Img<T, DP>;
+  static constexpr bool HELD = DP * T::ES <= 512;
+  uint4 f[HELD ? I::NC : 1];
+  const typename T::elem* p;
+  int D, h;
+  __device__ __forceinline__ void load(const typename T::elem* p_, int D_, int h_) {
+    p = p_, D = D_, h = h_;
+    if constexpr (HELD) {
+#pragma unroll
+      for (int j = 0; j < I::NC; ++j) f[j] = chunk(j);
+    }
+  }
+  __device__ __forceinline__ uint4 chunk(int j) const {
+    return p && (2 * j + h) * I::E < D ? ld_chunk<T>(p, 2 * j + h, D) : zero16();
+  }
+  __device__ __forceinline__ uint4 operator[](int j) const {
+    if constexpr (HELD)
+      return f[j];
+    else
+      return chunk(j);
+  }
+};
+
 // dQ of WR * 32 rows, streaming K and V; also delta (and the rows' |dO|) for
 // xattn_dkv, which runs after it.
 template <class T, int DP, int WR, int WS, int KT, int OCC>
 __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_dq(const XArgs a) {
   using I = Img<T, DP>;
-  using C = FwdCfg<T, DP, WR, WS, KT>;
+  using S = KeyStream<T, DP, WR, WS, KT>;
   using E = typename T::elem;
   const XWork w = x_work(a);
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wr = wave % WR, ws = wave / WR;
@@ -557,27 +732,23 @@ __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_dq(const XArgs a) {
   const int len = row0 < rows ? x_len(a.kv_lens, w.b, a.Tk) : 0;
   int klo, khi;
   x_share(len, KT, a.splits, w.split, klo, khi);
-  const uint8_t* mask = a.mask ? a.mask + w.b * a.mask_sb : nullptr;
-  const uint32_t LK = 0, LV = I::bytes(KT);
   const float c2 = a.scale * LOG2E_X;
   const long long at = (long long)w.bh * a.R;
 
-  uint4 qf[I::NC], df[I::NC];
+  Rows32<T, DP> qf, df;
   float delta = 0.f, amax = 0.f;
   {
     const bool live = row < rows;
-    const E* p = live ? x_row<E>(a.q, w.b, w.g, a.G, row) : nullptr;
-    const E* d = live ? x_row<E>(a.dout, w.b, w.g, a.G, row) : nullptr;
-    const E* o = live ? x_row<E>(a.o, w.b, w.g, a.G, row) : nullptr;
+    qf.load(live ? x_row<E>(a.q, w.b, w.g, a.G, row) : nullptr, a.D, h);
+    df.load(live ? x_row<E>(a.dout, w.b, w.g, a.G, row) : nullptr, a.D, h);
+    Rows32<T, DP> of;
+    of.p = live ? x_row<E>(a.o, w.b, w.g, a.G, row) : nullptr;
+    of.D = a.D, of.h = h;
 #pragma unroll
     for (int j = 0; j < I::NC; ++j) {
-      const int ch = 2 * j + h;
-      const bool in = live && ch * I::E < a.D;
-      qf[j] = in ? ld_chunk<T>(p, ch, a.D) : zero16();
-      df[j] = in ? ld_chunk<T>(d, ch, a.D) : zero16();
-      const uint4 ov = in ? ld_chunk<T>(o, ch, a.D) : zero16();
+      const uint4 dv = df[j], ov = of.chunk(j);
       E x[I::E], y[I::E];
-      __builtin_memcpy(x, &df[j], 16);
+      __builtin_memcpy(x, &dv, 16);
       __builtin_memcpy(y, &ov, 16);
 #pragma unroll
       for (int e = 0; e < I::E; ++e) {
@@ -590,54 +761,69 @@ __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_dq(const XArgs a) {
   amax = xhalf_max(amax);
   const float L = row < rows ? a.lse[at + row] : INFINITY;
   const float down = x_down<T>(amax);
+
+  // S and dP of a piece: s = P, returns dP
+  auto scores = [&](f32x16& s, uint32_t kb, const auto* ks, const auto* vs) {
+    f32x16 dp = {};
+    s = f32x16{};
+#pragma unroll
+    for (int j = 0; j < I::NC; ++j) {
+      s = T::mma(ks->rm(j), qf[j], s);
+      dp = T::mma(vs->rm(j), df[j], dp);
+    }
+    x_mask(s, kb, h);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -L));
+    return dp;
+  };
+  // With one tile of states, delta = sum P dP is summed from the products
+  // themselves: dO . O carries the rounding of O to the type, which few states
+  // do not average out (dQ was 1.53 times as far off as one rounding at 32
+  // states, against 1.42 times so).
+  if (T::ES == 2 && a.Tk <= KT) {
+    float sum = 0.f;
+    S::run(a, w, klo, khi, ws, [&](const uint32_t (&kb)[S::SUB], auto& ks, auto& vs) {
+#pragma unroll
+      for (int u = 0; u < S::SUB; ++u) {
+        f32x16 s;
+        const f32x16 dp = scores(s, kb[u], ks[u], vs[u]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum = fmaf(s[e], dp[e], sum);
+      }
+    });
+    sum = xhalf_sum(sum);
+    if constexpr (WS > 1) {
+      __syncthreads();
+      if (h == 0) lds_stf(4 * ((ws * WR + wr) * 32 + lr), sum);
+      __syncthreads();
+      sum = 0.f;
+      for (int x = 0; x < WS; ++x) sum += lds_ldf(4 * ((x * WR + wr) * 32 + lr));
+    }
+    if (L != INFINITY) delta = sum;
+  }
   if (w.split == 0 && ws == 0 && h == 0 && row < a.R) {
     a.delta[at + row] = delta;
     if (a.amax) a.amax[at + row] = amax;
   }
   f32x16 acc[DP / 32] = {};
-
-  Stage<T, DP, KT, C::NT> sk, sv;
-  Keep<KT> kp;
-  auto fetch = [&](int k0) {
-    kp.load(mask, k0, khi, lane);
-    sk.load([&](int r) { return k0 + r < khi ? x_key<E>(a.k, w.b, w.g, k0 + r) : nullptr; }, a.D);
-    sv.load([&](int r) { return k0 + r < khi ? x_key<E>(a.v, w.b, w.g, k0 + r) : nullptr; }, a.D);
-  };
-  if (klo < khi) fetch(klo);
-  for (int k0 = klo; k0 < khi; k0 += KT) {
-    uint64_t keep[Keep<KT>::W];
-    kp.bits(keep);
-    __syncthreads();
-    sk.store_kept(LK, keep);
-    sv.store_kept(LV, keep);
-    __syncthreads();
-    if (k0 + KT < khi) fetch(k0 + KT);
+  S::run(a, w, klo, khi, ws, [&](const uint32_t (&kb)[S::SUB], auto& ks, auto& vs) {
 #pragma unroll
-    for (int u = 0; u < C::SUB; ++u) {
-      const int r0 = (ws * C::SUB + u) * 32;
-      f32x16 s = {}, dp = {};
+    for (int u = 0; u < S::SUB; ++u) {
+      f32x16 s;
+      const f32x16 dp = scores(s, kb[u], ks[u], vs[u]);
 #pragma unroll
-      for (int j = 0; j < I::NC; ++j) {
-        s = T::mma(I::rm(LK, r0, j, lane), qf[j], s);
-        dp = T::mma(I::rm(LV, r0, j, lane), df[j], dp);
+      for (int e = 0; e < 16; ++e) {
+        s[e] *= dp[e] - delta;
+        if constexpr (std::is_same<T, XF16>::value) s[e] *= down;
       }
-      const uint32_t kb = (uint32_t)(keep[r0 >> 6] >> (r0 & 63));
-      if (kb != 0xffffffffu) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = (kb >> acc_row(e, h)) & 1 ? s[e] : -INFINITY;
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -L)) * ((dp[e] - delta) * down);
 #pragma unroll
       for (int c = 0; c < I::NPF; ++c) {
         const uint4 p = I::pack(s, c);
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
-          acc[db] = T::mma(I::tr(LK, r0, c, db, lane), p, acc[db]);
+        for (int db = 0; db < DP / 32; ++db) acc[db] = T::mma(ks[u]->tr(c, db), p, acc[db]);
       }
     }
-  }
+  });
   const float mul = a.scale / down;
   const bool none = L == INFINITY;
   if (a.splits == 1) {
@@ -659,7 +845,8 @@ template <class T, int DP, int WC, int WS, int DS, int RT>
 struct DkvCfg {
   static constexpr int NT = 64 * WC * WS * DS;
   static constexpr int SUB = RT / WS / 32;
-  static constexpr int ST = 2 * Img<T, DP>::bytes(RT);       // L, delta behind the tiles
+  static constexpr bool MEM = T::ES == 4;
+  static constexpr int ST = MEM ? 0 : 2 * Img<T, DP>::bytes(RT);   // L, delta behind the tiles
   static constexpr int OUT = x_store_bytes<T, DP / DS, WC, WS>();
   static constexpr int OUT32 = x_store_bytes<XF32, DP / DS, WC, WS>();
   static constexpr int LDS = x_max(ST + 8 * RT, DS * OUT);
@@ -682,7 +869,6 @@ __global__ __launch_bounds__(64 * WC * WS * DS, OCC) void xattn_dkv(const XArgs 
   int rlo, rhi;
   x_share(key0 < len ? rows : 0, RT, a.splits, w.split, rlo, rhi);
   const bool kept = key < len && (!a.mask || a.mask[w.b * a.mask_sb + key]);
-  const uint32_t LQ = 0, LD = I::bytes(RT), LL = C::ST, LT = LL + 4 * RT;
   const float c2 = a.scale * LOG2E_X;
   const long long at = (long long)w.bh * a.R;
 
@@ -698,71 +884,117 @@ __global__ __launch_bounds__(64 * WC * WS * DS, OCC) void xattn_dkv(const XArgs 
     __syncthreads();
   }
 
-  uint4 kf[I::NC], vf[I::NC];
-  {
-    const E* p = x_key<E>(a.k, w.b, w.g, kept ? key : 0);
-    const E* v = x_key<E>(a.v, w.b, w.g, kept ? key : 0);
-#pragma unroll
-    for (int j = 0; j < I::NC; ++j) {
-      const bool in = kept && (2 * j + h) * I::E < a.D;
-      kf[j] = in ? ld_chunk<T>(p, 2 * j + h, a.D) : zero16();
-      vf[j] = in ? ld_chunk<T>(v, 2 * j + h, a.D) : zero16();
-    }
-  }
+  Rows32<T, DP> kf, vf;
+  kf.load(kept ? x_key<E>(a.k, w.b, w.g, key) : nullptr, a.D, h);
+  vf.load(kept ? x_key<E>(a.v, w.b, w.g, key) : nullptr, a.D, h);
   f32x16 dk[NB] = {}, dv[NB] = {};
 
-  Stage<T, DP, RT, C::NT> sq, sd;
-  float fl = INFINITY, ft = 0.f;
-  auto fetch = [&](int r0) {
-    sq.load([&](int r) {
-      return r0 + r < rhi ? x_row<E>(a.q, w.b, w.g, a.G, r0 + r) : nullptr; }, a.D);
-    sd.load([&](int r) {
-      return r0 + r < rhi ? x_row<E>(a.dout, w.b, w.g, a.G, r0 + r) : nullptr; }, a.D);
-    const int r = r0 + threadIdx.x;
-    const bool in = threadIdx.x < RT && r < rhi;
-    fl = in ? a.lse[at + r] : INFINITY;
-    ft = in ? a.delta[at + r] : 0.f;
-  };
-  if (rlo < rhi) fetch(rlo);
-  for (int t0 = rlo; t0 < rhi; t0 += RT) {
-    __syncthreads();
-    sq.store(LQ);
-    sd.store(LD);
-    if (threadIdx.x < RT) {
-      lds_stf(LL + 4 * threadIdx.x, fl);
-      lds_stf(LT + 4 * threadIdx.x, ft);
+  // one piece of 32 rows: L and delta of row acc_row(4 k + e, h) in element e
+  // of stat(k)
+  auto piece = [&](const auto& qs, const auto& os, auto lse, auto del) {
+    f32x16 s = {}, dp = {};
+#pragma unroll
+    for (int j = 0; j < I::NC; ++j) {
+      s = T::mma(qs.rm(j), kf[j], s);
+      dp = T::mma(os.rm(j), vf[j], dp);
     }
-    __syncthreads();
-    if (t0 + RT < rhi) fetch(t0 + RT);
 #pragma unroll
-    for (int u = 0; u < C::SUB; ++u) {
-      const int r0 = (ws * C::SUB + u) * 32;
-      f32x16 s = {}, dp = {};
+    for (int k = 0; k < 4; ++k) {
+      const f32x4 L = lse(k), t = del(k);
 #pragma unroll
-      for (int j = 0; j < I::NC; ++j) {
-        s = T::mma(I::rm(LQ, r0, j, lane), kf[j], s);
-        dp = T::mma(I::rm(LD, r0, j, lane), vf[j], dp);
+      for (int e = 0; e < 4; ++e) {
+        const int i = 4 * k + e;
+        s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -L[e]));
+        dp[i] = s[i] * (dp[i] - t[e]);
+        if constexpr (std::is_same<T, XF16>::value) dp[i] *= down;
       }
+    }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint4 lu = lds_ld16(LL + 4 * (r0 + 8 * k + 4 * h));
-        const uint4 tu = lds_ld16(LT + 4 * (r0 + 8 * k + 4 * h));
-        const uint32_t *lp = (const uint32_t*)&lu, *tp = (const uint32_t*)&tu;
+    for (int c = 0; c < I::NPF; ++c) {
+      const uint4 p = I::pack(s, c), g = I::pack(dp, c);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = 4 * k + e;
-          s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -__uint_as_float(lp[e])));
-          dp[i] = s[i] * ((dp[i] - __uint_as_float(tp[e])) * down);
-        }
+      for (int db = 0; db < NB; ++db) {
+        dv[db] = T::mma(os.tr(c, ds * NB + db), p, dv[db]);
+        dk[db] = T::mma(qs.tr(c, ds * NB + db), g, dk[db]);
       }
+    }
+  };
+  // byte offset of row i of a tile that begins with a token's first head
+  auto in_tile = [&](const XView& v) {
+    const uint32_t st = (uint32_t)v.st * T::ES, sh = (uint32_t)v.sh * T::ES;
+    const int G = a.G;
+    return [=](int i) -> uint32_t {
+      const uint32_t t = G == 1 ? i : (unsigned)i / (unsigned)G;
+      return t * st + (i - t * G) * sh;
+    };
+  };
+  if constexpr (C::MEM) {
+    for (int r0 = rlo + 32 * ws; r0 < rhi; r0 += RT) {
+      const int n = rhi - r0;
+      const uint32_t live = n >= 32 ? 0xffffffffu : (1u << n) - 1;
+      // offsets from the first row's token
+      const int t0 = a.G == 1 ? r0 : (int)((unsigned)r0 / (unsigned)a.G), g0 = r0 - t0 * a.G;
+      MemSrc<DP> qs, os;
+      const auto qo = in_tile(a.q), oo = in_tile(a.dout);
+      qs.begin(x_row<E>(a.q, w.b, w.g, a.G, t0 * a.G), [&](int i) { return qo(g0 + i); }, live,
+               lane, a.D);
+      os.begin(x_row<E>(a.dout, w.b, w.g, a.G, t0 * a.G), [&](int i) { return oo(g0 + i); }, live,
+               lane, a.D);
+      auto stat = [&](const float* p, float none) {
+        return [=](int k) {
+          f32x4 v;
 #pragma unroll
-      for (int c = 0; c < I::NPF; ++c) {
-        const uint4 p = I::pack(s, c), g = I::pack(dp, c);
+          for (int e = 0; e < 4; ++e) {
+            const int i = 8 * k + 4 * h + e;
+            v[e] = i < n ? p[at + r0 + i] : none;
+          }
+          return v;
+        };
+      };
+      piece(qs, os, stat(a.lse, INFINITY), stat(a.delta, 0.f));
+    }
+  } else {
+    constexpr uint32_t LQ = 0, LD = I::bytes(RT), LL = C::ST, LT = LL + 4 * RT;
+    Stage<T, DP, RT, C::NT> sq, sd;
+    float fl = INFINITY, ft = 0.f;
+    sq.init(in_tile(a.q), a.D);
+    sd.init(in_tile(a.dout), a.D);
+    auto fetch = [&](int r0) {
+      if (a.fast_q) {       // G divides RT: a tile begins with a token's first head
+        sq.load(x_row<E>(a.q, w.b, w.g, a.G, r0), rhi - r0);
+        sd.load(x_row<E>(a.dout, w.b, w.g, a.G, r0), rhi - r0);
+      } else {
+        sq.load_any([&](int r) {
+          return r0 + r < rhi ? x_row<E>(a.q, w.b, w.g, a.G, r0 + r) : nullptr; }, a.D);
+        sd.load_any([&](int r) {
+          return r0 + r < rhi ? x_row<E>(a.dout, w.b, w.g, a.G, r0 + r) : nullptr; }, a.D);
+      }
+      const int r = r0 + threadIdx.x;
+      const bool in = threadIdx.x < RT && r < rhi;
+      fl = in ? a.lse[at + r] : INFINITY;
+      ft = in ? a.delta[at + r] : 0.f;
+    };
+    if (rlo < rhi) fetch(rlo);
+    for (int t0 = rlo; t0 < rhi; t0 += RT) {
+      __syncthreads();
+      sq.store(LQ);
+      sd.store(LD);
+      if (threadIdx.x < RT) {
+        lds_stf(LL + 4 * threadIdx.x, fl);
+        lds_stf(LT + 4 * threadIdx.x, ft);
+      }
+      __syncthreads();
+      if (t0 + RT < rhi) fetch(t0 + RT);
 #pragma unroll
-        for (int db = 0; db < NB; ++db) {
-          dv[db] = T::mma(I::tr(LD, r0, c, ds * NB + db, lane), p, dv[db]);
-          dk[db] = T::mma(I::tr(LQ, r0, c, ds * NB + db, lane), g, dk[db]);
-        }
+      for (int u = 0; u < C::SUB; ++u) {
+        const int r0 = (ws * C::SUB + u) * 32;
+        const LdsSrc<T, DP> qs{LQ + I::bytes(r0), lane}, os{LD + I::bytes(r0), lane};
+        auto stat = [&](uint32_t base) {
+          return [=](int k) {
+            return __builtin_bit_cast(f32x4, lds_ld16(base + 4 * (r0 + 8 * k + 4 * h)));
+          };
+        };
+        piece(qs, os, stat(LL), stat(LT));
       }
     }
   }
@@ -812,23 +1044,25 @@ __global__ __launch_bounds__(256) void xattn_join(const XArgs a) {
 enum { X_FWD, X_DQ, X_DKV };
 
 struct XPlan {
-  int few, tiles, splits;
+  int waves, tiles, splits;      // waves that own rows (dK, dV: states), 32 each
 };
 // The split of one kernel's work.  `own` rows (dK, dV: states) belong to the
-// waves, 32 each; the others are streamed.  Where 32 (fp32 with 256 columns:
-// 64) hold them all, the block's waves share them and take different parts of
-// the stream.  Fewer than 512 blocks (two per CU) split the stream further,
-// into parts that a second launch joins.
+// waves, the others are streamed.  A block's four waves own 32 rows each while
+// that leaves two blocks per CU; below, two or all four waves share rows and
+// take different parts of the stream, and below that the stream is split over
+// blocks, whose results a second launch joins.
 inline XPlan x_plan(const XArgs& a, int type, int what) {
   const int own = what == X_DKV ? a.Tk : a.R, stream = what == X_DKV ? a.R : a.Tk;
-  const bool wide = type == 1 && a.D > 128;
+  const long long heads = (long long)a.B * a.Hk;
+  const bool halves = what == X_DKV && type != 1 && a.D > 128;    // two waves per 32 states
   XPlan p;
-  p.few = own <= (wide && what != X_DKV ? 64 : 32);
-  const int per = wide && what == X_DKV ? 64 : 128;
-  p.tiles = p.few ? 1 : (own + per - 1) / per;
-  const long long blocks = (long long)p.tiles * a.B * a.Hk;
-  const int step = p.few ? 128 : 64, most = (stream + step - 1) / step;
-  const long long want = blocks >= 512 ? 1 : (512 + blocks - 1) / blocks;
+  for (p.waves = halves ? 2 : 4;; p.waves /= 2) {
+    p.tiles = (own + 32 * p.waves - 1) / (32 * p.waves);
+    if (p.waves == 1 || (p.tiles * heads >= 512 && own > 16 * p.waves)) break;
+  }
+  const long long blocks = p.tiles * heads;
+  const int most = (stream + 127) / 128;
+  const long long want = blocks >= 384 ? 1 : (512 + blocks - 1) / blocks;
   p.splits = (int)(want < most ? want : most);
   return p;
 }
@@ -842,48 +1076,53 @@ int x_go(K kernel, const XArgs& a, int lds, int nt, void* stream) {
   return (int)hipGetLastError();
 }
 
+template <class T, int DP, int W>
+int x_rows(const XArgs& a, int what, void* stream) {
+  // fp32 takes one piece of 32 states per wave; 16-bit tiles hold 64 states
+  // (32 for four waves of 256 columns: the registers), 128 where four waves
+  // share them
+  constexpr int KT = T::ES == 4 ? 32 * (4 / W) : W == 1 ? 128 : W == 4 && DP == 256 ? 32 : 64;
+  constexpr int OCC = DP * T::ES <= 256 && W > 1 ? 2 : 1;
+  using S = KeyStream<T, DP, W, 4 / W, KT>;
+  const int lds = a.splits > 1 ? S::LDS32 : S::LDS;
+  return what == X_FWD ? x_go(xattn_fwd<T, DP, W, 4 / W, KT, OCC>, a, lds, S::NT, stream)
+                       : x_go(xattn_dq<T, DP, W, 4 / W, KT, OCC>, a, lds, S::NT, stream);
+}
+template <class T, int DP, int W>
+int x_states(const XArgs& a, void* stream) {
+  constexpr int DS = T::ES == 2 && DP == 256 ? 2 : 1, WS = 4 / DS / W;
+  using C = DkvCfg<T, DP, W, WS, DS, 32 * WS>;
+  return x_go(xattn_dkv<T, DP, W, WS, DS, 32 * WS, 1>, a, a.splits > 1 ? C::LDS32 : C::LDS, C::NT,
+              stream);
+}
+
 template <class T, int DP>
 int x_run(XArgs a, int what, void* stream) {
-  constexpr bool wide = DP * T::ES > 512;               // fp32, 256 columns
-  constexpr int OCC = DP * T::ES <= 256 ? 2 : 1;
-  constexpr int KT = wide ? 32 : 64;
-  constexpr int FR = wide ? 2 : 1, FS = wide ? 2 : 4, FK = wide ? 64 : 128;
   const XPlan p = x_plan(a, T::TYPE, what);
   a.tiles = p.tiles;
   a.splits = p.splits;
   const int nrow = a.B * a.Hk * (what == X_DKV ? a.Tk : a.R);
   int e;
-  if (what != X_DKV) {
-    using C = FwdCfg<T, DP, 4, 1, KT>;
-    using S = FwdCfg<T, DP, FR, FS, FK>;
-    constexpr int L = x_max(C::LDS, x_store_bytes<XF32, DP, 4, 1>());
-    const int lds = p.few ? S::LDS : a.splits > 1 ? L : C::LDS;
-    if (what == X_FWD) {
-      e = p.few ? x_go(xattn_fwd<T, DP, FR, FS, FK, 1>, a, lds, S::NT, stream)
-                : x_go(xattn_fwd<T, DP, 4, 1, KT, OCC>, a, lds, C::NT, stream);
-      if (e || a.splits == 1) return e;
-      hipLaunchKernelGGL((xattn_fwd_join<T>), dim3((nrow + 3) / 4), dim3(256), 0,
-                         (hipStream_t)stream, a);
-      return (int)hipGetLastError();
-    }
-    e = p.few ? x_go(xattn_dq<T, DP, FR, FS, FK, 1>, a, lds, S::NT, stream)
-              : x_go(xattn_dq<T, DP, 4, 1, KT, OCC>, a, lds, C::NT, stream);
-    if (e || a.splits == 1) return e;
-    hipLaunchKernelGGL((xattn_join<T, false>), dim3((nrow + 3) / 4), dim3(256), 0,
-                       (hipStream_t)stream, a);
-    return (int)hipGetLastError();
+  if (what == X_DKV) {
+    if constexpr (T::ES == 2 && DP == 256)
+      e = p.waves == 2 ? x_states<T, DP, 2>(a, stream) : x_states<T, DP, 1>(a, stream);
+    else
+      e = p.waves == 4   ? x_states<T, DP, 4>(a, stream)
+          : p.waves == 2 ? x_states<T, DP, 2>(a, stream)
+                         : x_states<T, DP, 1>(a, stream);
+  } else {
+    e = p.waves == 4   ? x_rows<T, DP, 4>(a, what, stream)
+        : p.waves == 2 ? x_rows<T, DP, 2>(a, what, stream)
+                       : x_rows<T, DP, 1>(a, what, stream);
   }
-  constexpr int DS = wide ? 2 : 1, RT = 32;
-  constexpr int MC = wide ? 2 : 4;                        // states: 32 MC per block
-  using C = DkvCfg<T, DP, MC, 1, DS, RT>;
-  using S = DkvCfg<T, DP, 1, MC, DS, 32 * MC>;
-  e = p.few ? x_go(xattn_dkv<T, DP, 1, MC, DS, 32 * MC, 1>, a, a.splits > 1 ? S::LDS32 : S::LDS,
-                   S::NT, stream)
-            : x_go(xattn_dkv<T, DP, MC, 1, DS, RT, 1>, a, a.splits > 1 ? C::LDS32 : C::LDS, C::NT,
-                   stream);
   if (e || a.splits == 1) return e;
-  hipLaunchKernelGGL((xattn_join<T, true>), dim3((nrow + 3) / 4, 2), dim3(256), 0,
-                     (hipStream_t)stream, a);
+  const dim3 grid((nrow + 3) / 4, what == X_DKV ? 2 : 1);
+  if (what == X_FWD)
+    hipLaunchKernelGGL((xattn_fwd_join<T>), grid, dim3(256), 0, (hipStream_t)stream, a);
+  else if (what == X_DQ)
+    hipLaunchKernelGGL((xattn_join<T, false>), grid, dim3(256), 0, (hipStream_t)stream, a);
+  else
+    hipLaunchKernelGGL((xattn_join<T, true>), grid, dim3(256), 0, (hipStream_t)stream, a);
   return (int)hipGetLastError();
 }
 

@@ -36,6 +36,24 @@ long long x_part(const XArgs& a, int type, int what) {
   return n * a.D * (kv ? 2 : 1) + (what == X_FWD ? 2 * n : 0);
 }
 
+// The kernels read tiles of up to 128 rows by 32-bit offsets from the first.
+bool x_span(const XArgs& a, const XView& v, int type, int heads) {
+  const long long es = type == 1 ? 4 : 2;
+  return v.st >= 0 && v.sh >= 0 && (160 * v.st + heads * v.sh + 256) * es < 1LL << 31;
+}
+// Whole chunks of 16 bytes at 4-byte alignment.
+bool x_chunks(const XArgs& a, const XView& v) {
+  return a.D % 8 == 0 && !((uintptr_t)v.p & 3) && !((v.sb | v.st | v.sh) & 1);
+}
+int x_reading(XArgs& a, int type) {
+  if (!x_span(a, a.q, type, a.G) || !x_span(a, a.k, type, 1) || !x_span(a, a.v, type, 1) ||
+      (a.dout.p && !x_span(a, a.dout, type, a.G)))
+    return 1001;
+  a.fast_k = x_chunks(a, a.k) && x_chunks(a, a.v);
+  a.fast_q = x_chunks(a, a.q) && x_chunks(a, a.dout) && 32 % a.G == 0;
+  return 0;
+}
+
 XView view(const void* p, const long long* s) { return XView{(void*)p, s[0], s[1], s[2]}; }
 
 }  // namespace
@@ -70,6 +88,7 @@ int tgfr_cross_attention_fwd(const void* q, const void* k, const void* v, void* 
   a.k = view(k, strides + 3);
   a.v = view(v, strides + 6);
   a.o = view(o, strides + 9);
+  if (const int e = x_reading(a, type)) return e;
   a.q_lens = q_lens;
   a.kv_lens = kv_lens;
   a.mask = mask;
@@ -100,6 +119,7 @@ int tgfr_cross_attention_bwd(const void* q, const void* k, const void* v, const 
   a.o = view(o, strides + 9);
   a.dout = view(dout, strides + 12);
   a.dq = view(dq, strides + 15);
+  if (const int e = x_reading(a, type)) return e;
   a.q_lens = q_lens;
   a.kv_lens = kv_lens;
   a.mask = mask;
