@@ -194,62 +194,68 @@ __device__ __forceinline__ uint32_t buf4(__amdgpu_buffer_rsrc_t r, uint32_t off)
   return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
 }
 
-// A tile of ROWS rows (16-bit types) in flight from global memory to LDS, held
-// in registers.  A thread's chunks lie at fixed offsets from the tile's first
-// row, so a whole tile costs no address arithmetic but the scalar base's.
+// Feeds tiles of ROWS rows (16-bit types) to LDS images by DMA, which takes no
+// registers: a wave's instruction fills 1 KiB of the image in lane order, so
+// the lanes fetch the chunks that the image's swizzle puts there.  A thread's
+// chunks lie at fixed offsets from the tile's first row: a whole tile costs no
+// address arithmetic but the scalar base's.
 template <class T, int DP, int ROWS, int NT>
-struct Stage {
+struct Feed {
   using I = Img<T, DP>;
-  static constexpr int N = ROWS * I::CPR / NT, STEP = NT / I::CPR;
-  static_assert(ROWS * I::CPR % NT == 0 && NT % I::CPR == 0, "whole rows per step");
-  uint4 r[N];
+  static constexpr int N = ROWS * I::CPR / NT;
+  static_assert(ROWS * I::CPR % NT == 0, "whole instructions");
   uint32_t off[N];
+  bool whole;            // every chunk of the image is part of a row
+
+  static __device__ __forceinline__ int row(int n) { return (threadIdx.x + NT * n) / I::CPR; }
+  static __device__ __forceinline__ int chunk(int n) {
+    return (int)(threadIdx.x + NT * n) % I::CPR ^ I::f(row(n));
+  }
+  static __device__ __forceinline__ uint32_t place(int n) { return 16 * (threadIdx.x + NT * n); }
 
   // at(i): byte offset of row i from the tile's first
   template <class At>
   __device__ __forceinline__ void init(At at, int D) {
-    const int ch = threadIdx.x % I::CPR;
+    whole = D == DP;
 #pragma unroll
     for (int n = 0; n < N; ++n)
-      off[n] = ch * I::E < D ? at(threadIdx.x / I::CPR + STEP * n) + 16 * ch : NONE;
+      off[n] = chunk(n) * I::E < D ? at(row(n)) + 16 * chunk(n) : NONE;
   }
-  // the tile whose first row is at p, `rows` of them (at least 1)
-  __device__ __forceinline__ void load(const void* p, int rows) {
-    const __amdgpu_buffer_rsrc_t b = tile_rsrc(p);
-    if (rows >= ROWS) {
+  // columns past D, once: the feed leaves them alone
+  __device__ __forceinline__ void clear(uint32_t base) const {
+    if (whole) return;
 #pragma unroll
-      for (int n = 0; n < N; ++n) r[n] = buf16(b, off[n]);
+    for (int n = 0; n < N; ++n)
+      if (off[n] == NONE) lds_st16(base + place(n), zero16());
+  }
+  // starts a tile whose first row is at p, of `rows` rows (at least 1)
+  __device__ __forceinline__ void start(const void* p, int rows, uint32_t base) const {
+    const uint32_t to = base + 16 * (threadIdx.x & ~63u);
+    if (whole && rows >= ROWS) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) glds16s(p, off[n], to + 16 * NT * n);
     } else {
 #pragma unroll
       for (int n = 0; n < N; ++n)
-        r[n] = buf16(b, (int)threadIdx.x / I::CPR + STEP * n < rows ? off[n] : NONE);
+        if (off[n] != NONE && row(n) < rows) glds16s(p, off[n], to + 16 * NT * n);
     }
   }
-  // rows at any alignment and of any length: row(i) points to row i of the
-  // tile, or is NULL for zeros
+  // the same for rows at any alignment and of any length, through registers:
+  // at(i) points to row i of the tile, or is NULL for zeros
   template <class Row>
-  __device__ __forceinline__ void load_any(Row row, int D) {
-    const int ch = threadIdx.x % I::CPR;
+  __device__ __forceinline__ void copy(Row at, int D, uint32_t base) const {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const typename T::elem* p = row(threadIdx.x / I::CPR + STEP * n);
-      r[n] = p && ch * I::E < D ? ld_chunk<T>(p, ch, D) : zero16();
+      const typename T::elem* p = at(row(n));
+      lds_st16(base + place(n), p && chunk(n) * I::E < D ? ld_chunk<T>(p, chunk(n), D) : zero16());
     }
   }
-  __device__ __forceinline__ void store(uint32_t base) const {
+  // zeros in the rows that gone(row) names
+  template <class Gone>
+  __device__ __forceinline__ void drop(Gone gone, uint32_t base) const {
 #pragma unroll
     for (int n = 0; n < N; ++n)
-      lds_st16(base + I::at(threadIdx.x / I::CPR + STEP * n, threadIdx.x % I::CPR), r[n]);
-  }
-  // zeros where keep has no bit
-  template <int W>
-  __device__ __forceinline__ void store_kept(uint32_t base, const uint64_t (&keep)[W]) const {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int row = threadIdx.x / I::CPR + STEP * n;
-      const bool k = (keep[W == 1 ? 0 : row >> 6] >> (row & 63)) & 1;
-      lds_st16(base + I::at(row, threadIdx.x % I::CPR), k ? r[n] : zero16());
-    }
+      if (gone(row(n))) lds_st16(base + place(n), zero16());
   }
 };
 
@@ -265,16 +271,16 @@ struct LdsSrc {
     return I::tr(base, 0, c, db, lane);
   }
 };
-// fp32: straight from global memory.  Its matrix instructions take 16 times as
-// long per byte as bf16's, so cache and load latency hide behind them without
-// a tile in LDS, without barriers, and with no registers for tiles in flight.
+// fp32: straight from global memory.  Its matrix instructions take 8 times as
+// long per byte as bf16's, so cache reads hide behind them without a tile in
+// LDS; what counts is loads in flight, so a wave takes 64 columns (below).
 template <int DP>
 struct MemSrc {
   __amdgpu_buffer_rsrc_t b;
   uint32_t row, tro[16];
   int lane, D;
-  // the 32 rows whose first is at p; at(i): byte offset of row i; bit i of
-  // `live`: row i exists (others are zeros)
+  // the 32 rows whose first is at p (D: elements from there on); at(i): byte
+  // offset of row i; bit i of `live`: row i exists (others are zeros)
   template <class At>
   __device__ __forceinline__ void begin(const void* p, At at, uint32_t live, int lane_, int D_) {
     lane = lane_;
@@ -448,82 +454,100 @@ constexpr int x_max(int a, int b) { return a > b ? a : b; }
 // ------------------------------------------------------------ the key stream ---
 // The states of a split, KT at a time, as the forward and dQ read them: WR
 // waves along the rows (32 each) x WS waves along the states of a tile, SUB
-// pieces of 32 states per wave and tile.
-template <class T, int DP, int WR, int WS, int KT>
+// pieces of 32 states per wave and tile, x DS waves along the columns.
+//
+// fp32 with more than 64 columns: DS waves take 64 columns each of Q, K, V and
+// the result.  Each forms its part of the scores, the parts are exchanged
+// through LDS and summed by all in one order (1/8 of the time of the products
+// they belong to), so a wave's operands and accumulators are a quarter of 256
+// columns' and its loads stay in flight.
+template <class T, int DP, int WR, int WS, int DS, int KT>
 struct KeyStream {
   using I = Img<T, DP>;
   using E = typename T::elem;
-  static constexpr int NT = 64 * WR * WS, SUB = KT / WS / 32;
+  static constexpr int NT = 64 * WR * WS * DS, SUB = KT / WS / 32, DH = DP / DS;
   static constexpr bool MEM = T::ES == 4;
-  static constexpr int TILES = MEM ? 0 : 2 * I::bytes(KT);
-  static constexpr int ML = x_max(TILES, x_store_bytes<T, DP, WR, WS>());
-  // behind the tiles: 2 floats per row and wave
-  static constexpr int LDS = ML + 2 * 4 * 32 * WR * WS;
-  static constexpr int LDS32 = x_max(TILES, x_store_bytes<XF32, DP, WR, WS>()) +
-                               2 * 4 * 32 * WR * WS;
+  static constexpr int TILE = MEM ? 0 : 2 * I::bytes(KT);
+  // two tiles (fp32: two exchanges of 8 KiB per wave), later the result
+  static constexpr int FED = MEM ? (DS > 1 ? 2 * 8192 * WR * WS * DS : 0) : 2 * TILE;
+  static constexpr int STAT = 2 * 4 * 32 * WR * WS;
+  static constexpr int OUT = x_store_bytes<T, DH, WR, WS>();
+  static constexpr int OUT32 = x_store_bytes<XF32, DH, WR, WS>();
+  static constexpr int LDS = x_max(x_max(FED, DS * OUT), STAT);
+  static constexpr int LDS32 = x_max(x_max(FED, DS * OUT32), STAT);
 
-  // f(piece u, its kept bits, K source, V source) for every piece of 32 states
-  // that this wave handles; all waves of the block take part.  post(): after
-  // the tile's pieces.
+  // f(kept bits, K sources, V sources), one of each per piece of 32 states,
+  // for every tile; all waves of the block take part.
   template <class F>
   static __device__ __forceinline__ void run(const XArgs& a, const XWork& w, int klo, int khi,
-                                             int ws, F f) {
+                                             int ws, int ds, F f) {
     const int lane = threadIdx.x % 64;
     const uint8_t* mask = a.mask ? a.mask + w.b * a.mask_sb : nullptr;
-    const E* K = x_key<E>(a.k, w.b, w.g, 0);
-    const E* V = x_key<E>(a.v, w.b, w.g, 0);
+    const E* K = x_key<E>(a.k, w.b, w.g, 0) + ds * DH;
+    const E* V = x_key<E>(a.v, w.b, w.g, 0) + ds * DH;
     const uint32_t kst = (uint32_t)a.k.st * T::ES, vst = (uint32_t)a.v.st * T::ES;
     if constexpr (MEM) {
       static_assert(SUB == 1, "one piece per wave");
-      for (int k0 = klo + 32 * ws; k0 < khi; k0 += KT) {
-        const int j = k0 + (lane & 31);
+      for (int t0 = klo; t0 < khi; t0 += KT) {
+        const int k0 = t0 + 32 * ws, j = k0 + (lane & 31);
         const uint32_t kb = (uint32_t)__ballot(j < khi && (!mask || mask[j]));
-        MemSrc<DP> ks, vs;
-        ks.begin(K + k0 * a.k.st, [&](int r) { return r * kst; }, kb, lane, a.D);
-        vs.begin(V + k0 * a.v.st, [&](int r) { return r * vst; }, kb, lane, a.D);
-        const MemSrc<DP>*kp[1] = {&ks}, *vp[1] = {&vs};
+        if (DS == 1 && !kb) continue;
+        MemSrc<DH> ks, vs;
+        ks.begin(K + k0 * a.k.st, [&](int r) { return r * kst; }, kb, lane, a.D - ds * DH);
+        vs.begin(V + k0 * a.v.st, [&](int r) { return r * vst; }, kb, lane, a.D - ds * DH);
+        const MemSrc<DH>*kp[1] = {&ks}, *vp[1] = {&vs};
         const uint32_t kbs[1] = {kb};
         f(kbs, kp, vp);
       }
     } else {
-      constexpr uint32_t LK = 0, LV = I::bytes(KT);
-      Stage<T, DP, KT, NT> sk, sv;
+      static_assert(DS == 1, "whole rows");
+      constexpr uint32_t V0 = I::bytes(KT);
+      Feed<T, DP, KT, NT> fk, fv;
       Keep<KT> kp;
-      sk.init([&](int r) { return r * kst; }, a.D);
-      sv.init([&](int r) { return r * vst; }, a.D);
-      auto fetch = [&](int k0) {
-        kp.load(mask, k0, khi, lane);
+      fk.init([&](int r) { return r * kst; }, a.D);
+      fv.init([&](int r) { return r * vst; }, a.D);
+      __syncthreads();                   // the LDS may have been in use
+      for (uint32_t l0 = 0; l0 < 2 * TILE; l0 += TILE) {
+        fk.clear(l0);
+        fv.clear(l0 + V0);
+      }
+      auto start = [&](int k0, uint32_t l0) {
         if (a.fast_k) {
-          sk.load(K + k0 * a.k.st, khi - k0);
-          sv.load(V + k0 * a.v.st, khi - k0);
+          fk.start(K + k0 * a.k.st, khi - k0, l0);
+          fv.start(V + k0 * a.v.st, khi - k0, l0 + V0);
         } else {
-          sk.load_any([&](int r) { return k0 + r < khi ? K + (k0 + r) * a.k.st : nullptr; }, a.D);
-          sv.load_any([&](int r) { return k0 + r < khi ? V + (k0 + r) * a.v.st : nullptr; }, a.D);
+          fk.copy([&](int r) { return k0 + r < khi ? K + (k0 + r) * a.k.st : nullptr; }, a.D, l0);
+          fv.copy([&](int r) { return k0 + r < khi ? V + (k0 + r) * a.v.st : nullptr; }, a.D,
+                  l0 + V0);
         }
       };
-      if (klo < khi) fetch(klo);
-      for (int k0 = klo; k0 < khi; k0 += KT) {
+      // The tile behind the current one is fed while this one is worked on;
+      // its mask is loaded a tile earlier still, so that waiting for it does
+      // not wait for a feed.
+      kp.load(mask, klo, khi, lane);
+      if (klo < khi) start(klo, 0);
+      uint32_t l0 = 0;
+      for (int k0 = klo; k0 < khi; k0 += KT, l0 ^= TILE) {
+        ring_barrier<0>();
         uint64_t keep[Keep<KT>::W];
         const bool all = kp.bits(keep);
-        __syncthreads();
-        if (all) {
-          sk.store(LK);
-          sv.store(LV);
-        } else {
-          sk.store_kept(LK, keep);
-          sv.store_kept(LV, keep);
+        if (!all) {
+          auto gone = [&](int r) { return !((keep[KT <= 64 ? 0 : r >> 6] >> (r & 63)) & 1); };
+          fk.drop(gone, l0);
+          fv.drop(gone, l0 + V0);
+          __syncthreads();
         }
-        __syncthreads();
-        if (k0 + KT < khi) fetch(k0 + KT);
+        kp.load(mask, k0 + KT, khi, lane);
+        if (k0 + KT < khi) start(k0 + KT, l0 ^ TILE);
         uint32_t kbs[SUB];
         LdsSrc<T, DP> ks[SUB], vs[SUB];
         const LdsSrc<T, DP>*kq[SUB], *vq[SUB];
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
           const int r0 = (ws * SUB + u) * 32;
-          kbs[u] = (uint32_t)(keep[r0 >> 6] >> (r0 & 63));
-          ks[u] = {LK + I::bytes(r0), lane};
-          vs[u] = {LV + I::bytes(r0), lane};
+          kbs[u] = (uint32_t)(keep[KT <= 64 ? 0 : r0 >> 6] >> (r0 & 63));
+          ks[u] = {l0 + I::bytes(r0), lane};
+          vs[u] = {l0 + V0 + I::bytes(r0), lane};
           kq[u] = &ks[u];
           vq[u] = &vs[u];
         }
@@ -531,6 +555,50 @@ struct KeyStream {
       }
     }
   }
+};
+
+// Sums a score tile over the DS waves that formed parts of it (N tiles per
+// exchange); `turn` alternates between two places, so one barrier is enough.
+template <int DS, int N>
+__device__ __forceinline__ void x_exchange(f32x16 (&s)[N], int group, int ds, int& turn) {
+  if constexpr (DS > 1) {
+    const int lane = threadIdx.x % 64;
+    const uint32_t base = (turn * (int)(blockDim.x / 64) + group * DS) * 8192 + 16 * lane;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        lds_st16(base + ds * 8192 + 4096 * n + 1024 * k,
+                 make_uint4(__float_as_uint(s[n][4 * k]), __float_as_uint(s[n][4 * k + 1]),
+                            __float_as_uint(s[n][4 * k + 2]), __float_as_uint(s[n][4 * k + 3])));
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        f32x4 v = __builtin_bit_cast(f32x4, lds_ld16(base + 4096 * n + 1024 * k));
+#pragma unroll
+        for (int x = 1; x < DS; ++x)
+          v += __builtin_bit_cast(f32x4, lds_ld16(base + x * 8192 + 4096 * n + 1024 * k));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][4 * k + e] = v[e];
+      }
+    turn ^= 1;
+  }
+}
+
+// B operands of 32 rows, one per lane, held in registers.
+template <class T, int DP>
+struct Rows32 {
+  using I = Img<T, DP>;
+  uint4 f[I::NC];
+  // p: the lane's row, or NULL for zeros, of D elements
+  __device__ __forceinline__ void load(const typename T::elem* p, int D, int h) {
+#pragma unroll
+    for (int j = 0; j < I::NC; ++j)
+      f[j] = p && (2 * j + h) * I::E < D ? ld_chunk<T>(p, 2 * j + h, D) : zero16();
+  }
+  __device__ __forceinline__ const uint4& operator[](int j) const { return f[j]; }
 };
 
 // scores of masked states
@@ -542,13 +610,14 @@ __device__ __forceinline__ void x_mask(f32x16& s, uint32_t kb, int h) {
 }
 
 // ------------------------------------------------------------------ forward ---
-template <class T, int DP, int WR, int WS, int KT, int OCC>
-__global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_fwd(const XArgs a) {
-  using I = Img<T, DP>;
-  using S = KeyStream<T, DP, WR, WS, KT>;
+template <class T, int DP, int WR, int WS, int DS, int KT, int OCC>
+__global__ __launch_bounds__(64 * WR * WS * DS, OCC) void xattn_fwd(const XArgs a) {
+  using S = KeyStream<T, DP, WR, WS, DS, KT>;
+  using I = Img<T, S::DH>;
   using E = typename T::elem;
   const XWork w = x_work(a);
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wr = wave % WR, ws = wave / WR;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int wr = wave % WR, ws = wave / WR % WS, ds = wave / (WR * WS);
   const int lr = lane & 31, h = lane >> 5;
   const int rows = x_len(a.q_lens, w.b, a.Tq) * a.G;
   const int row0 = w.tile * WR * 32, row = row0 + wr * 32 + lr;
@@ -557,21 +626,18 @@ __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_fwd(const XArgs a) {
   x_share(len, KT, a.splits, w.split, klo, khi);
   const float c2 = a.scale * LOG2E_X;
 
-  uint4 qf[I::NC];
-  {
-    const E* p = row < rows ? x_row<E>(a.q, w.b, w.g, a.G, row) : nullptr;
-#pragma unroll
-    for (int j = 0; j < I::NC; ++j)
-      qf[j] = p && (2 * j + h) * I::E < a.D ? ld_chunk<T>(p, 2 * j + h, a.D) : zero16();
-  }
-  f32x16 acc[DP / 32] = {};
+  const int Dh = a.D - ds * S::DH;           // columns from this wave's first on
+  Rows32<T, S::DH> qf;
+  qf.load(row < rows ? x_row<E>(a.q, w.b, w.g, a.G, row) + ds * S::DH : nullptr, Dh, h);
+  f32x16 acc[S::DH / 32] = {};
+  int turn = 0;
   // the reference that exponents are taken against, in the log2 domain:
   // exp(scale s - max) = 2^(c2 s - m).  It follows the running maximum only
   // once that has grown by 8: sums and accumulators, relative to it, stay
   // exact, probabilities stay below 2^8, and most tiles rescale nothing.
   float m = -INFINITY, l = 0.f;
 
-  S::run(a, w, klo, khi, ws, [&](const uint32_t (&kb)[S::SUB], auto& ks, auto& vs) {
+  S::run(a, w, klo, khi, ws, ds, [&](const uint32_t (&kb)[S::SUB], auto& ks, auto& vs) {
     f32x16 s[S::SUB];
     float top = -INFINITY;
 #pragma unroll
@@ -579,6 +645,10 @@ __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_fwd(const XArgs a) {
       s[u] = f32x16{};
 #pragma unroll
       for (int j = 0; j < I::NC; ++j) s[u] = T::mma(ks[u]->rm(j), qf[j], s[u]);
+    }
+    x_exchange<DS>(s, ws * WR + wr, ds, turn);
+#pragma unroll
+    for (int u = 0; u < S::SUB; ++u) {
       x_mask(s[u], kb[u], h);
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
@@ -590,7 +660,7 @@ __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_fwd(const XArgs a) {
       m = mn;
       l *= al;
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db) acc[db] *= al;
+      for (int db = 0; db < S::DH / 32; ++db) acc[db] *= al;
     }
     const float mu = m == -INFINITY ? 0.f : m;        // no kept state so far
 #pragma unroll
@@ -604,7 +674,7 @@ __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_fwd(const XArgs a) {
       for (int c = 0; c < I::NPF; ++c) {
         const uint4 p = I::pack(s[u], c);
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) acc[db] = T::mma(vs[u]->tr(c, db), p, acc[db]);
+        for (int db = 0; db < S::DH / 32; ++db) acc[db] = T::mma(vs[u]->tr(c, db), p, acc[db]);
       }
     }
   });
@@ -614,7 +684,7 @@ __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_fwd(const XArgs a) {
   if constexpr (WS > 1) {       // the waves that share rows agree on the reference
     constexpr uint32_t ML = 0;
     __syncthreads();
-    if (h == 0) {
+    if (h == 0 && ds == 0) {
       lds_stf(ML + 4 * ((ws * WR + wr) * 32 + lr), m);
       lds_stf(ML + 4 * ((WS * WR + ws * WR + wr) * 32 + lr), l);
     }
@@ -630,21 +700,22 @@ __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_fwd(const XArgs a) {
     l = ll;
   }
   const bool none = !(row < rows) || (m == -INFINITY && l == 0.f);
+  const int tid = threadIdx.x % (64 * WR * WS);
   const long long at = (long long)w.bh * a.R;
   if (a.splits == 1) {
-    if (a.lse && ws == 0 && h == 0 && row < a.R)
+    if (a.lse && ws == 0 && ds == 0 && h == 0 && row < a.R)
       a.lse[at + row] = none ? INFINITY : m + __builtin_amdgcn_logf(l);
-    x_store<T, DP, WR, WS>(acc, mul / l, none, a.D, threadIdx.x, 0, [&](int r) -> E* {
-      return row0 + r < a.R ? x_row<E>(a.o, w.b, w.g, a.G, row0 + r) : nullptr;
+    x_store<T, S::DH, WR, WS>(acc, mul / l, none, Dh, tid, ds * S::OUT, [&](int r) -> E* {
+      return row0 + r < a.R ? x_row<E>(a.o, w.b, w.g, a.G, row0 + r) + ds * S::DH : nullptr;
     });
   } else {
     const long long ps = ((long long)w.split * a.B * a.Hk + w.bh) * a.R;
-    if (ws == 0 && h == 0 && row < a.R) {
+    if (ws == 0 && ds == 0 && h == 0 && row < a.R) {
       a.part_ml[2 * (ps + row)] = none ? -INFINITY : m;
       a.part_ml[2 * (ps + row) + 1] = none ? 0.f : l;
     }
-    x_store<XF32, DP, WR, WS>(acc, mul, none, a.D, threadIdx.x, 0, [&](int r) -> float* {
-      return row0 + r < a.R ? a.part + (ps + row0 + r) * a.D : nullptr;
+    x_store<XF32, S::DH, WR, WS>(acc, mul, none, Dh, tid, ds * S::OUT32, [&](int r) -> float* {
+      return row0 + r < a.R ? a.part + (ps + row0 + r) * a.D + ds * S::DH : nullptr;
     });
   }
 }
@@ -690,42 +761,16 @@ __device__ __forceinline__ float x_down(float amax) {
   return 1.f;
 }
 
-// B operands of 32 rows (one per lane): held in registers, or, where two of
-// them would fill the registers (fp32, 256 columns), read at each use.
-template <class T, int DP>
-struct Rows32 {
-  using I = Img<T, DP>;
-  static constexpr bool HELD = DP * T::ES <= 512;
-  uint4 f[HELD ? I::NC : 1];
-  const typename T::elem* p;
-  int D, h;
-  __device__ __forceinline__ void load(const typename T::elem* p_, int D_, int h_) {
-    p = p_, D = D_, h = h_;
-    if constexpr (HELD) {
-#pragma unroll
-      for (int j = 0; j < I::NC; ++j) f[j] = chunk(j);
-    }
-  }
-  __device__ __forceinline__ uint4 chunk(int j) const {
-    return p && (2 * j + h) * I::E < D ? ld_chunk<T>(p, 2 * j + h, D) : zero16();
-  }
-  __device__ __forceinline__ uint4 operator[](int j) const {
-    if constexpr (HELD)
-      return f[j];
-    else
-      return chunk(j);
-  }
-};
-
 // dQ of WR * 32 rows, streaming K and V; also delta (and the rows' |dO|) for
 // xattn_dkv, which runs after it.
-template <class T, int DP, int WR, int WS, int KT, int OCC>
-__global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_dq(const XArgs a) {
-  using I = Img<T, DP>;
-  using S = KeyStream<T, DP, WR, WS, KT>;
+template <class T, int DP, int WR, int WS, int DS, int KT, int OCC>
+__global__ __launch_bounds__(64 * WR * WS * DS, OCC) void xattn_dq(const XArgs a) {
+  using S = KeyStream<T, DP, WR, WS, DS, KT>;
+  using I = Img<T, S::DH>;
   using E = typename T::elem;
   const XWork w = x_work(a);
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wr = wave % WR, ws = wave / WR;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int wr = wave % WR, ws = wave / WR % WS, ds = wave / (WR * WS);
   const int lr = lane & 31, h = lane >> 5;
   const int rows = x_len(a.q_lens, w.b, a.Tq) * a.G;
   const int row0 = w.tile * WR * 32, row = row0 + wr * 32 + lr;
@@ -735,18 +780,18 @@ __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_dq(const XArgs a) {
   const float c2 = a.scale * LOG2E_X;
   const long long at = (long long)w.bh * a.R;
 
-  Rows32<T, DP> qf, df;
+  const int Dh = a.D - ds * S::DH;           // columns from this wave's first on
+  Rows32<T, S::DH> qf, df;
   float delta = 0.f, amax = 0.f;
   {
     const bool live = row < rows;
-    qf.load(live ? x_row<E>(a.q, w.b, w.g, a.G, row) : nullptr, a.D, h);
-    df.load(live ? x_row<E>(a.dout, w.b, w.g, a.G, row) : nullptr, a.D, h);
-    Rows32<T, DP> of;
-    of.p = live ? x_row<E>(a.o, w.b, w.g, a.G, row) : nullptr;
-    of.D = a.D, of.h = h;
+    const E* o = live ? x_row<E>(a.o, w.b, w.g, a.G, row) + ds * S::DH : nullptr;
+    qf.load(live ? x_row<E>(a.q, w.b, w.g, a.G, row) + ds * S::DH : nullptr, Dh, h);
+    df.load(live ? x_row<E>(a.dout, w.b, w.g, a.G, row) + ds * S::DH : nullptr, Dh, h);
 #pragma unroll
     for (int j = 0; j < I::NC; ++j) {
-      const uint4 dv = df[j], ov = of.chunk(j);
+      const uint4 dv = df[j];
+      const uint4 ov = o && (2 * j + h) * I::E < Dh ? ld_chunk<T>(o, 2 * j + h, Dh) : zero16();
       E x[I::E], y[I::E];
       __builtin_memcpy(x, &dv, 16);
       __builtin_memcpy(y, &ov, 16);
@@ -759,22 +804,29 @@ __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_dq(const XArgs a) {
   }
   delta = xhalf_sum(delta);
   amax = xhalf_max(amax);
+  if constexpr (DS > 1) {                      // of all columns
+    lds_stf(4 * (wave * 32 + lr), delta);
+    __syncthreads();
+    delta = 0.f;
+    for (int x = 0; x < DS; ++x) delta += lds_ldf(4 * (((x * WS + ws) * WR + wr) * 32 + lr));
+    __syncthreads();
+  }
   const float L = row < rows ? a.lse[at + row] : INFINITY;
   const float down = x_down<T>(amax);
+  int turn = 0;
 
-  // S and dP of a piece: s = P, returns dP
-  auto scores = [&](f32x16& s, uint32_t kb, const auto* ks, const auto* vs) {
-    f32x16 dp = {};
-    s = f32x16{};
+  // P of a piece in sp[0], dP in sp[1]
+  auto scores = [&](f32x16 (&sp)[2], uint32_t kb, const auto* ks, const auto* vs) {
+    sp[0] = sp[1] = f32x16{};
 #pragma unroll
     for (int j = 0; j < I::NC; ++j) {
-      s = T::mma(ks->rm(j), qf[j], s);
-      dp = T::mma(vs->rm(j), df[j], dp);
+      sp[0] = T::mma(ks->rm(j), qf[j], sp[0]);
+      sp[1] = T::mma(vs->rm(j), df[j], sp[1]);
     }
-    x_mask(s, kb, h);
+    x_exchange<DS>(sp, ws * WR + wr, ds, turn);
+    x_mask(sp[0], kb, h);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -L));
-    return dp;
+    for (int e = 0; e < 16; ++e) sp[0][e] = __builtin_amdgcn_exp2f(fmaf(sp[0][e], c2, -L));
   };
   // With one tile of states, delta = sum P dP is summed from the products
   // themselves: dO . O carries the rounding of O to the type, which few states
@@ -782,13 +834,13 @@ __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_dq(const XArgs a) {
   // states, against 1.42 times so).
   if (T::ES == 2 && a.Tk <= KT) {
     float sum = 0.f;
-    S::run(a, w, klo, khi, ws, [&](const uint32_t (&kb)[S::SUB], auto& ks, auto& vs) {
+    S::run(a, w, klo, khi, ws, ds, [&](const uint32_t (&kb)[S::SUB], auto& ks, auto& vs) {
 #pragma unroll
       for (int u = 0; u < S::SUB; ++u) {
-        f32x16 s;
-        const f32x16 dp = scores(s, kb[u], ks[u], vs[u]);
+        f32x16 sp[2];
+        scores(sp, kb[u], ks[u], vs[u]);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sum = fmaf(s[e], dp[e], sum);
+        for (int e = 0; e < 16; ++e) sum = fmaf(sp[0][e], sp[1][e], sum);
       }
     });
     sum = xhalf_sum(sum);
@@ -801,64 +853,69 @@ __global__ __launch_bounds__(64 * WR * WS, OCC) void xattn_dq(const XArgs a) {
     }
     if (L != INFINITY) delta = sum;
   }
-  if (w.split == 0 && ws == 0 && h == 0 && row < a.R) {
+  if (w.split == 0 && ws == 0 && ds == 0 && h == 0 && row < a.R) {
     a.delta[at + row] = delta;
     if (a.amax) a.amax[at + row] = amax;
   }
-  f32x16 acc[DP / 32] = {};
-  S::run(a, w, klo, khi, ws, [&](const uint32_t (&kb)[S::SUB], auto& ks, auto& vs) {
+  f32x16 acc[S::DH / 32] = {};
+  S::run(a, w, klo, khi, ws, ds, [&](const uint32_t (&kb)[S::SUB], auto& ks, auto& vs) {
 #pragma unroll
     for (int u = 0; u < S::SUB; ++u) {
-      f32x16 s;
-      const f32x16 dp = scores(s, kb[u], ks[u], vs[u]);
+      f32x16 sp[2];
+      scores(sp, kb[u], ks[u], vs[u]);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        s[e] *= dp[e] - delta;
-        if constexpr (std::is_same<T, XF16>::value) s[e] *= down;
+        sp[0][e] *= sp[1][e] - delta;
+        if constexpr (std::is_same<T, XF16>::value) sp[0][e] *= down;
       }
 #pragma unroll
       for (int c = 0; c < I::NPF; ++c) {
-        const uint4 p = I::pack(s, c);
+        const uint4 p = I::pack(sp[0], c);
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) acc[db] = T::mma(ks[u]->tr(c, db), p, acc[db]);
+        for (int db = 0; db < S::DH / 32; ++db) acc[db] = T::mma(ks[u]->tr(c, db), p, acc[db]);
       }
     }
   });
   const float mul = a.scale / down;
   const bool none = L == INFINITY;
+  const int tid = threadIdx.x % (64 * WR * WS);
   if (a.splits == 1) {
-    x_store<T, DP, WR, WS>(acc, mul, none, a.D, threadIdx.x, 0, [&](int r) -> E* {
-      return row0 + r < a.R ? x_row<E>(a.dq, w.b, w.g, a.G, row0 + r) : nullptr;
+    x_store<T, S::DH, WR, WS>(acc, mul, none, Dh, tid, ds * S::OUT, [&](int r) -> E* {
+      return row0 + r < a.R ? x_row<E>(a.dq, w.b, w.g, a.G, row0 + r) + ds * S::DH : nullptr;
     });
   } else {
     const long long ps = ((long long)w.split * a.B * a.Hk + w.bh) * a.R;
-    x_store<XF32, DP, WR, WS>(acc, mul, none, a.D, threadIdx.x, 0, [&](int r) -> float* {
-      return row0 + r < a.R ? a.part + (ps + row0 + r) * a.D : nullptr;
+    x_store<XF32, S::DH, WR, WS>(acc, mul, none, Dh, tid, ds * S::OUT32, [&](int r) -> float* {
+      return row0 + r < a.R ? a.part + (ps + row0 + r) * a.D + ds * S::DH : nullptr;
     });
   }
 }
 
 // dK and dV of WC * 32 states, streaming Q and dO over RT rows at a time; WS
 // waves share the states and take different rows, DS waves the columns of the
-// results (where both accumulators are too large for one wave's registers).
+// results: of fp32 as above, of 16-bit types with 256 columns because both
+// accumulators are too large for one wave's registers (each of the two forms
+// all of the scores, 6 products where 4 would do).
 template <class T, int DP, int WC, int WS, int DS, int RT>
 struct DkvCfg {
   static constexpr int NT = 64 * WC * WS * DS;
   static constexpr int SUB = RT / WS / 32;
   static constexpr bool MEM = T::ES == 4;
-  static constexpr int ST = MEM ? 0 : 2 * Img<T, DP>::bytes(RT);   // L, delta behind the tiles
+  static constexpr int TILE = MEM ? 0 : 2 * Img<T, DP>::bytes(RT) + 8 * RT;   // Q, dO, L, delta
+  static constexpr int FED = MEM ? (DS > 1 ? 2 * 8192 * WC * WS * DS : 0) : 2 * TILE;
   static constexpr int OUT = x_store_bytes<T, DP / DS, WC, WS>();
   static constexpr int OUT32 = x_store_bytes<XF32, DP / DS, WC, WS>();
-  static constexpr int LDS = x_max(ST + 8 * RT, DS * OUT);
+  static constexpr int LDS = x_max(x_max(FED, DS * OUT), 64);
   static constexpr int LDS32 = x_max(LDS, DS * OUT32);
 };
 
 template <class T, int DP, int WC, int WS, int DS, int RT, int OCC>
 __global__ __launch_bounds__(64 * WC * WS * DS, OCC) void xattn_dkv(const XArgs a) {
-  using I = Img<T, DP>;
   using C = DkvCfg<T, DP, WC, WS, DS, RT>;
+  // operands: a wave's own columns (fp32) or all
+  constexpr int DH = DP / DS, NB = DH / 32, DO = C::MEM ? DH : DP;
+  using I = Img<T, DO>;
   using E = typename T::elem;
-  constexpr int DH = DP / DS, NB = DH / 32;
   const XWork w = x_work(a);
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const int wc = wave % WC, ws = wave / WC % WS, ds = wave / (WC * WS);
@@ -884,38 +941,42 @@ __global__ __launch_bounds__(64 * WC * WS * DS, OCC) void xattn_dkv(const XArgs 
     __syncthreads();
   }
 
-  Rows32<T, DP> kf, vf;
-  kf.load(kept ? x_key<E>(a.k, w.b, w.g, key) : nullptr, a.D, h);
-  vf.load(kept ? x_key<E>(a.v, w.b, w.g, key) : nullptr, a.D, h);
+  const int c0 = C::MEM ? ds * DH : 0;         // first column of the operands
+  Rows32<T, DO> kf, vf;
+  kf.load(kept ? x_key<E>(a.k, w.b, w.g, key) + c0 : nullptr, a.D - c0, h);
+  vf.load(kept ? x_key<E>(a.v, w.b, w.g, key) + c0 : nullptr, a.D - c0, h);
   f32x16 dk[NB] = {}, dv[NB] = {};
+  int turn = 0;
 
   // one piece of 32 rows: L and delta of row acc_row(4 k + e, h) in element e
   // of stat(k)
   auto piece = [&](const auto& qs, const auto& os, auto lse, auto del) {
-    f32x16 s = {}, dp = {};
+    f32x16 sp[2] = {};
 #pragma unroll
     for (int j = 0; j < I::NC; ++j) {
-      s = T::mma(qs.rm(j), kf[j], s);
-      dp = T::mma(os.rm(j), vf[j], dp);
+      sp[0] = T::mma(qs.rm(j), kf[j], sp[0]);
+      sp[1] = T::mma(os.rm(j), vf[j], sp[1]);
     }
+    if constexpr (C::MEM) x_exchange<DS>(sp, ws * WC + wc, ds, turn);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const f32x4 L = lse(k), t = del(k);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = 4 * k + e;
-        s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -L[e]));
-        dp[i] = s[i] * (dp[i] - t[e]);
-        if constexpr (std::is_same<T, XF16>::value) dp[i] *= down;
+        sp[0][i] = __builtin_amdgcn_exp2f(fmaf(sp[0][i], c2, -L[e]));
+        sp[1][i] = sp[0][i] * (sp[1][i] - t[e]);
+        if constexpr (std::is_same<T, XF16>::value) sp[1][i] *= down;
       }
     }
+    const int b0 = C::MEM ? 0 : ds * NB;
 #pragma unroll
     for (int c = 0; c < I::NPF; ++c) {
-      const uint4 p = I::pack(s, c), g = I::pack(dp, c);
+      const uint4 p = I::pack(sp[0], c), g = I::pack(sp[1], c);
 #pragma unroll
       for (int db = 0; db < NB; ++db) {
-        dv[db] = T::mma(os.tr(c, ds * NB + db), p, dv[db]);
-        dk[db] = T::mma(qs.tr(c, ds * NB + db), g, dk[db]);
+        dv[db] = T::mma(os.tr(c, b0 + db), p, dv[db]);
+        dk[db] = T::mma(qs.tr(c, b0 + db), g, dk[db]);
       }
     }
   };
@@ -929,17 +990,18 @@ __global__ __launch_bounds__(64 * WC * WS * DS, OCC) void xattn_dkv(const XArgs 
     };
   };
   if constexpr (C::MEM) {
-    for (int r0 = rlo + 32 * ws; r0 < rhi; r0 += RT) {
-      const int n = rhi - r0;
-      const uint32_t live = n >= 32 ? 0xffffffffu : (1u << n) - 1;
+    for (int t = rlo; t < rhi; t += RT) {
+      const int r0 = t + 32 * ws, n = rhi - r0;
+      const uint32_t live = n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1 : 0u;
+      if (DS == 1 && !live) continue;
       // offsets from the first row's token
       const int t0 = a.G == 1 ? r0 : (int)((unsigned)r0 / (unsigned)a.G), g0 = r0 - t0 * a.G;
-      MemSrc<DP> qs, os;
+      MemSrc<DO> qs, os;
       const auto qo = in_tile(a.q), oo = in_tile(a.dout);
-      qs.begin(x_row<E>(a.q, w.b, w.g, a.G, t0 * a.G), [&](int i) { return qo(g0 + i); }, live,
-               lane, a.D);
-      os.begin(x_row<E>(a.dout, w.b, w.g, a.G, t0 * a.G), [&](int i) { return oo(g0 + i); }, live,
-               lane, a.D);
+      qs.begin(x_row<E>(a.q, w.b, w.g, a.G, t0 * a.G) + c0, [&](int i) { return qo(g0 + i); },
+               live, lane, a.D - c0);
+      os.begin(x_row<E>(a.dout, w.b, w.g, a.G, t0 * a.G) + c0, [&](int i) { return oo(g0 + i); },
+               live, lane, a.D - c0);
       auto stat = [&](const float* p, float none) {
         return [=](int k) {
           f32x4 v;
@@ -954,47 +1016,59 @@ __global__ __launch_bounds__(64 * WC * WS * DS, OCC) void xattn_dkv(const XArgs 
       piece(qs, os, stat(a.lse, INFINITY), stat(a.delta, 0.f));
     }
   } else {
-    constexpr uint32_t LQ = 0, LD = I::bytes(RT), LL = C::ST, LT = LL + 4 * RT;
-    Stage<T, DP, RT, C::NT> sq, sd;
+    constexpr uint32_t D0 = I::bytes(RT), L0 = 2 * D0, T0 = L0 + 4 * RT;
+    Feed<T, DP, RT, C::NT> fq, fd;
+    fq.init(in_tile(a.q), a.D);
+    fd.init(in_tile(a.dout), a.D);
+    for (uint32_t l0 = 0; l0 < 2 * C::TILE; l0 += C::TILE) {
+      fq.clear(l0);
+      fd.clear(l0 + D0);
+    }
     float fl = INFINITY, ft = 0.f;
-    sq.init(in_tile(a.q), a.D);
-    sd.init(in_tile(a.dout), a.D);
-    auto fetch = [&](int r0) {
-      if (a.fast_q) {       // G divides RT: a tile begins with a token's first head
-        sq.load(x_row<E>(a.q, w.b, w.g, a.G, r0), rhi - r0);
-        sd.load(x_row<E>(a.dout, w.b, w.g, a.G, r0), rhi - r0);
-      } else {
-        sq.load_any([&](int r) {
-          return r0 + r < rhi ? x_row<E>(a.q, w.b, w.g, a.G, r0 + r) : nullptr; }, a.D);
-        sd.load_any([&](int r) {
-          return r0 + r < rhi ? x_row<E>(a.dout, w.b, w.g, a.G, r0 + r) : nullptr; }, a.D);
-      }
+    auto stats = [&](int r0) {
       const int r = r0 + threadIdx.x;
       const bool in = threadIdx.x < RT && r < rhi;
       fl = in ? a.lse[at + r] : INFINITY;
       ft = in ? a.delta[at + r] : 0.f;
     };
-    if (rlo < rhi) fetch(rlo);
-    for (int t0 = rlo; t0 < rhi; t0 += RT) {
-      __syncthreads();
-      sq.store(LQ);
-      sd.store(LD);
+    auto start = [&](int r0, uint32_t l0) {
       if (threadIdx.x < RT) {
-        lds_stf(LL + 4 * threadIdx.x, fl);
-        lds_stf(LT + 4 * threadIdx.x, ft);
+        lds_stf(l0 + L0 + 4 * threadIdx.x, fl);
+        lds_stf(l0 + T0 + 4 * threadIdx.x, ft);
       }
-      __syncthreads();
-      if (t0 + RT < rhi) fetch(t0 + RT);
+      stats(r0 + RT);       // of the tile after: waiting for it then waits for no feed
+      if (a.fast_q) {       // G divides RT: a tile begins with a token's first head
+        fq.start(x_row<E>(a.q, w.b, w.g, a.G, r0), rhi - r0, l0);
+        fd.start(x_row<E>(a.dout, w.b, w.g, a.G, r0), rhi - r0, l0 + D0);
+      } else {
+        fq.copy([&](int r) {
+          return r0 + r < rhi ? x_row<E>(a.q, w.b, w.g, a.G, r0 + r) : nullptr; }, a.D, l0);
+        fd.copy([&](int r) {
+          return r0 + r < rhi ? x_row<E>(a.dout, w.b, w.g, a.G, r0 + r) : nullptr; }, a.D, l0 + D0);
+      }
+    };
+    stats(rlo);
+    if (rlo < rhi) start(rlo, 0);
+    uint32_t l0 = 0;
+    for (int t0 = rlo; t0 < rhi; t0 += RT, l0 ^= C::TILE) {
+      ring_barrier<0>();
+      if (t0 + RT > rhi) {
+        auto gone = [&](int r) { return t0 + r >= rhi; };
+        fq.drop(gone, l0);
+        fd.drop(gone, l0 + D0);
+        __syncthreads();
+      }
+      if (t0 + RT < rhi) start(t0 + RT, l0 ^ C::TILE);
 #pragma unroll
       for (int u = 0; u < C::SUB; ++u) {
         const int r0 = (ws * C::SUB + u) * 32;
-        const LdsSrc<T, DP> qs{LQ + I::bytes(r0), lane}, os{LD + I::bytes(r0), lane};
+        const LdsSrc<T, DP> qs{l0 + I::bytes(r0), lane}, os{l0 + D0 + I::bytes(r0), lane};
         auto stat = [&](uint32_t base) {
           return [=](int k) {
             return __builtin_bit_cast(f32x4, lds_ld16(base + 4 * (r0 + 8 * k + 4 * h)));
           };
         };
-        piece(qs, os, stat(LL), stat(LT));
+        piece(qs, os, stat(l0 + L0), stat(l0 + T0));
       }
     }
   }
@@ -1046,22 +1120,34 @@ enum { X_FWD, X_DQ, X_DKV };
 struct XPlan {
   int waves, tiles, splits;      // waves that own rows (dK, dV: states), 32 each
 };
+// Waves along the columns: fp32 64 columns each; dK, dV of 16-bit types with
+// 256 columns two waves.
+constexpr int x_columns(int type, int what, int dp) {
+  return type == 1 ? dp / 64 : what == X_DKV && dp == 256 ? 2 : 1;
+}
+// least waves along the rows
+constexpr int x_least(int type, int what, int dp) {
+  return type != 1 && what != X_DKV && dp == 256 ? 2 : 1;
+}
 // The split of one kernel's work.  `own` rows (dK, dV: states) belong to the
-// waves, the others are streamed.  A block's four waves own 32 rows each while
-// that leaves two blocks per CU; below, two or all four waves share rows and
-// take different parts of the stream, and below that the stream is split over
+// waves, the others are streamed.  A block's four waves (or those that the
+// columns leave) own 32 rows each while that leaves two blocks per CU; below,
+// two or all of them share rows and take different parts of the stream, where
+// that has a piece of 32 for each, and below that the stream is split over
 // blocks, whose results a second launch joins.
 inline XPlan x_plan(const XArgs& a, int type, int what) {
   const int own = what == X_DKV ? a.Tk : a.R, stream = what == X_DKV ? a.R : a.Tk;
   const long long heads = (long long)a.B * a.Hk;
-  const bool halves = what == X_DKV && type != 1 && a.D > 128;    // two waves per 32 states
+  const int dp = a.D <= 64 ? 64 : a.D <= 128 ? 128 : 256, all = 4 / x_columns(type, what, dp);
   XPlan p;
-  for (p.waves = halves ? 2 : 4;; p.waves /= 2) {
+  for (p.waves = all;; p.waves /= 2) {
     p.tiles = (own + 32 * p.waves - 1) / (32 * p.waves);
-    if (p.waves == 1 || (p.tiles * heads >= 512 && own > 16 * p.waves)) break;
+    if (p.waves == x_least(type, what, dp) || (p.tiles * heads >= 512 && own > 16 * p.waves) ||
+        stream <= 32 * (all / p.waves))
+      break;
   }
   const long long blocks = p.tiles * heads;
-  const int most = (stream + 127) / 128;
+  const int step = type == 1 ? 32 * (all / p.waves) : 128, most = (stream + step - 1) / step;
   const long long want = blocks >= 384 ? 1 : (512 + blocks - 1) / blocks;
   p.splits = (int)(want < most ? want : most);
   return p;
@@ -1078,22 +1164,35 @@ int x_go(K kernel, const XArgs& a, int lds, int nt, void* stream) {
 
 template <class T, int DP, int W>
 int x_rows(const XArgs& a, int what, void* stream) {
-  // fp32 takes one piece of 32 states per wave; 16-bit tiles hold 64 states
-  // (32 for four waves of 256 columns: the registers), 128 where four waves
-  // share them
-  constexpr int KT = T::ES == 4 ? 32 * (4 / W) : W == 1 ? 128 : W == 4 && DP == 256 ? 32 : 64;
-  constexpr int OCC = DP * T::ES <= 256 && W > 1 ? 2 : 1;
-  using S = KeyStream<T, DP, W, 4 / W, KT>;
+  // fp32 takes one piece of 32 states per wave; 16-bit tiles hold 64 states,
+  // 128 where four waves share them (of 256 columns two such tiles would pass
+  // the LDS: x_least)
+  constexpr int DS = x_columns(T::TYPE, X_FWD, DP), WS = 4 / DS / W;
+  constexpr int KT = T::ES == 4 ? 32 * WS : W == 1 ? 128 : 64;
+  constexpr int OCC = T::ES == 4 ? 2 : DP <= 128 && W > 1 ? 2 : 1;
+  using S = KeyStream<T, DP, W, WS, DS, KT>;
   const int lds = a.splits > 1 ? S::LDS32 : S::LDS;
-  return what == X_FWD ? x_go(xattn_fwd<T, DP, W, 4 / W, KT, OCC>, a, lds, S::NT, stream)
-                       : x_go(xattn_dq<T, DP, W, 4 / W, KT, OCC>, a, lds, S::NT, stream);
+  return what == X_FWD ? x_go(xattn_fwd<T, DP, W, WS, DS, KT, OCC>, a, lds, S::NT, stream)
+                       : x_go(xattn_dq<T, DP, W, WS, DS, KT, OCC>, a, lds, S::NT, stream);
 }
 template <class T, int DP, int W>
 int x_states(const XArgs& a, void* stream) {
-  constexpr int DS = T::ES == 2 && DP == 256 ? 2 : 1, WS = 4 / DS / W;
+  constexpr int DS = x_columns(T::TYPE, X_DKV, DP), WS = 4 / DS / W;
   using C = DkvCfg<T, DP, W, WS, DS, 32 * WS>;
   return x_go(xattn_dkv<T, DP, W, WS, DS, 32 * WS, 1>, a, a.splits > 1 ? C::LDS32 : C::LDS, C::NT,
               stream);
+}
+template <class T, int DP, int W>
+int x_waves(const XArgs& a, int waves, int what, void* stream) {
+  if constexpr (W > 1)
+    if (waves < W) return x_waves<T, DP, W / 2>(a, waves, what, stream);
+  if (what == X_DKV) {
+    if constexpr (W * x_columns(T::TYPE, X_DKV, DP) <= 4) return x_states<T, DP, W>(a, stream);
+  } else {
+    if constexpr (W * x_columns(T::TYPE, X_FWD, DP) <= 4 && W >= x_least(T::TYPE, X_FWD, DP))
+      return x_rows<T, DP, W>(a, what, stream);
+  }
+  return 1001;
 }
 
 template <class T, int DP>
@@ -1102,19 +1201,7 @@ int x_run(XArgs a, int what, void* stream) {
   a.tiles = p.tiles;
   a.splits = p.splits;
   const int nrow = a.B * a.Hk * (what == X_DKV ? a.Tk : a.R);
-  int e;
-  if (what == X_DKV) {
-    if constexpr (T::ES == 2 && DP == 256)
-      e = p.waves == 2 ? x_states<T, DP, 2>(a, stream) : x_states<T, DP, 1>(a, stream);
-    else
-      e = p.waves == 4   ? x_states<T, DP, 4>(a, stream)
-          : p.waves == 2 ? x_states<T, DP, 2>(a, stream)
-                         : x_states<T, DP, 1>(a, stream);
-  } else {
-    e = p.waves == 4   ? x_rows<T, DP, 4>(a, what, stream)
-        : p.waves == 2 ? x_rows<T, DP, 2>(a, what, stream)
-                       : x_rows<T, DP, 1>(a, what, stream);
-  }
+  const int e = x_waves<T, DP, 4>(a, p.waves, what, stream);
   if (e || a.splits == 1) return e;
   const dim3 grid((nrow + 3) / 4, what == X_DKV ? 2 : 1);
   if (what == X_FWD)
