@@ -33,6 +33,11 @@
 
 namespace tgfr {
 
+#define X_INLINE __attribute__((always_inline))
+// waves per SIMD, neither fewer nor more: a compiler that hopes for more keeps
+// registers free that operands read ahead need
+#define X_OCCUPANCY(n) __attribute__((amdgpu_waves_per_eu(n, n)))
+
 constexpr float LOG2E_X = 1.4426950408889634f;
 
 // element strides of a [B][T][H][D] tensor with unit stride over D
@@ -194,6 +199,27 @@ __device__ __forceinline__ uint32_t buf4(__amdgpu_buffer_rsrc_t r, uint32_t off)
   return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
 }
 
+// 16 (4) bytes per lane from a scalar base + lane offset straight to LDS byte
+// `to` (wave-uniform) + 16 (4) * lane.  Inline asm, so that the compiler sees no
+// LDS write pending on the memory counter; the kernels wait by count (glds16).
+__device__ __forceinline__ const void* scalar(const void* p) {
+  const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)p);
+  const uint64_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)((uintptr_t)p >> 32));
+  return (const void*)(lo | (hi << 32));
+}
+__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t to) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_base() + to));
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off),
+               "s"(scalar(base)), "s"(m0)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t to) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_base() + to));
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off),
+               "s"(scalar(base)), "s"(m0)
+               : "memory", "m0");
+}
+
 // Feeds tiles of ROWS rows (16-bit types) to LDS images by DMA, which takes no
 // registers: a wave's instruction fills 1 KiB of the image in lane order, so
 // the lanes fetch the chunks that the image's swizzle puts there.  A thread's
@@ -228,16 +254,19 @@ struct Feed {
     for (int n = 0; n < N; ++n)
       if (off[n] == NONE) lds_st16(base + place(n), zero16());
   }
-  // starts a tile whose first row is at p, of `rows` rows (at least 1)
+  // starts a whole tile (FULL), or one of `rows` rows, whose first is at p: N
+  // DMA instructions per wave for a whole tile
+  template <bool FULL>
   __device__ __forceinline__ void start(const void* p, int rows, uint32_t base) const {
     const uint32_t to = base + 16 * (threadIdx.x & ~63u);
-    if (whole && rows >= ROWS) {
-#pragma unroll
-      for (int n = 0; n < N; ++n) glds16s(p, off[n], to + 16 * NT * n);
-    } else {
+    if (whole) {
 #pragma unroll
       for (int n = 0; n < N; ++n)
-        if (off[n] != NONE && row(n) < rows) glds16s(p, off[n], to + 16 * NT * n);
+        if (FULL || row(n) < rows) dma16(p, off[n], to + 16 * NT * n);
+    } else {       // an instruction covers whole rows: some lanes always take part
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (off[n] != NONE && (FULL || row(n) < rows)) dma16(p, off[n], to + 16 * NT * n);
     }
   }
   // the same for rows at any alignment and of any length, through registers:
@@ -317,8 +346,13 @@ struct XWork {
   int b, g, bh, tile, split;
 };
 __device__ __forceinline__ XWork x_work(const XArgs& a) {
-  // consecutive work shares K and V (or Q and dO), and so one XCD's L2
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  // Consecutive work shares K and V (or Q and dO), and so one XCD's L2.  With
+  // lengths, whole samples per XCD would leave the XCDs of short ones idle:
+  // they get runs of four.
+  const int total = gridDim.x, L = blockIdx.x, q = L / 8;
+  const int id = !(a.q_lens || a.kv_lens) ? xcd_remap(L, total)
+                 : L < total / 32 * 32    ? (q / 4 * 8 + L % 8) * 4 + q % 4
+                                          : L;
   XWork w;
   w.tile = id % a.tiles;
   const int rest = id / a.tiles;
@@ -326,6 +360,8 @@ __device__ __forceinline__ XWork x_work(const XArgs& a) {
   w.split = rest / (a.B * a.Hk);
   w.b = w.bh / a.Hk;
   w.g = w.bh % a.Hk;
+  // (division runs on the vector unit; these are the same in all lanes)
+  for (int* p : {&w.tile, &w.bh, &w.split, &w.b, &w.g}) *p = __builtin_amdgcn_readfirstlane(*p);
   return w;
 }
 __device__ __forceinline__ int x_len(const int* lens, int b, int T) {
@@ -343,33 +379,9 @@ __device__ __forceinline__ E* x_key(const XView& v, int b, int g, int j) {
 // [first, last) of a split's share of n items in whole tiles
 __device__ __forceinline__ void x_share(int n, int tile, int splits, int split, int& lo, int& hi) {
   const int nt = (n + tile - 1) / tile, per = (nt + splits - 1) / splits;
-  lo = min(n, split * per * tile);
-  hi = min(n, (split + 1) * per * tile);
+  lo = __builtin_amdgcn_readfirstlane(min(n, split * per * tile));
+  hi = __builtin_amdgcn_readfirstlane(min(n, (split + 1) * per * tile));
 }
-// which of the tile's states are attended to, one bit each, equal in all waves
-template <int KT>
-struct Keep {
-  static constexpr int W = (KT + 63) / 64;
-  uint8_t m[W];
-  __device__ __forceinline__ void load(const uint8_t* mask, int k0, int len, int lane) {
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const int j = k0 + 64 * w + lane;
-      m[w] = 64 * w + lane < KT && j < len ? (mask ? mask[j] : 1) : 0;
-    }
-  }
-  // true: the whole tile
-  __device__ __forceinline__ bool bits(uint64_t (&keep)[W]) const {
-    bool all = true;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      keep[w] = __ballot(m[w] != 0);
-      all = all && keep[w] == (KT < 64 ? (1ull << (KT % 64)) - 1 : ~0ull);
-    }
-    return all;
-  }
-};
-
 // Writes WR * 32 rows of DP accumulated values (acc[db][q]: column
 // 32 db + acc_row(q, h) of the wave's row lane % 32), summed over the WS waves
 // that share the rows, times mul, through LDS at `lb`, so that whole rows are
@@ -452,42 +464,135 @@ constexpr int x_store_bytes() {
 constexpr int x_max(int a, int b) { return a > b ? a : b; }
 
 // ------------------------------------------------------------ the key stream ---
-// The states of a split, KT at a time, as the forward and dQ read them: WR
-// waves along the rows (32 each) x WS waves along the states of a tile, SUB
-// pieces of 32 states per wave and tile, x DS waves along the columns.
+// The states of a split, a tile of KT = 32 WS at a time, as the forward and dQ
+// read them: WR waves along the rows (32 each) x WS waves along the states of
+// a tile (a piece of 32 each) x DS waves along the columns.
 //
 // fp32 with more than 64 columns: DS waves take 64 columns each of Q, K, V and
 // the result.  Each forms its part of the scores, the parts are exchanged
 // through LDS and summed by all in one order (1/8 of the time of the products
 // they belong to), so a wave's operands and accumulators are a quarter of 256
 // columns' and its loads stay in flight.
-template <class T, int DP, int WR, int WS, int DS, int KT>
+// One step in the order in which it is to run: RM products of the scores (of
+// the piece ahead), whose operands rm(i) are read AHEAD products early and
+// beside which beside(i) runs (the vector work of the current piece), then TR
+// products with operands tr(i).  (The compiler keeps this order where
+// accumulators fill the registers; written plainly, it read each operand right
+// before its product, and dK, dV took 2.5 times as long.)
+template <int RM, int TR, int AHEAD, class Rm, class Mma1, class Beside, class Between, class Tr,
+          class Mma2>
+__device__ __forceinline__ void x_step(Rm rm, Mma1 mma1, Beside beside, Between between, Tr tr,
+                                       Mma2 mma2) {
+  uint4 f[AHEAD];
+  auto load = [&](int i) X_INLINE { return i < RM ? rm(i) : tr(i - RM); };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (i < RM + TR) f[i] = load(i);
+#pragma unroll
+  for (int i = 0; i < RM; ++i) {
+    mma1(i, f[i % AHEAD]);
+    if (i + AHEAD < RM + TR) f[i % AHEAD] = load(i + AHEAD);
+    beside(i);
+  }
+  between();
+#pragma unroll
+  for (int i = RM; i < RM + TR; ++i) {
+    mma2(i - RM, f[i % AHEAD]);
+    if (i + AHEAD < RM + TR) f[i % AHEAD] = load(i + AHEAD);
+  }
+}
+struct XNone {
+  template <class... A>
+  __device__ __forceinline__ void operator()(A&&...) const {}
+};
+struct XNoOperand {
+  __device__ __forceinline__ uint4 operator()(int) const { return uint4{}; }
+};
+
+// The ring of four slots in LDS that 16-bit kernels stream through: piece n
+// lies in slot n % 4.  Step n forms the scores of piece n + 1 beside the rest
+// of piece n, so that matrix and vector instructions of one wave have
+// independent work to overlap; pieces n + 2 and n + 3 are being fed meanwhile.
+//   wait(n): piece n + 1 has arrived, all waves are past step n - 1; feeds n + 3
+//   first(sp, slot): scores of the piece there;  before(sp, n): what branches
+//   on them;  step(sp, slot, next, slot): the rest of a piece and the scores
+//   of the next;  last(sp, slot): the rest
+// PLAIN steps (whole tiles, nothing masked: `plain` of them) come four at a
+// time with constant slots, so that LDS addresses cost nothing.
+template <int N, class Wait, class First, class Before, class Step, class Last>
+__device__ __forceinline__ void x_pipe(int np, int plain, Wait wait, First first, Before before,
+                                       Step step, Last last) {
+  using Any = std::false_type;
+  using Plain = std::true_type;
+  if (np <= 0) return;
+  f32x16 now[N], next[N];
+  wait(-1, Any{});
+  first(now, 0);
+  int n = 0;
+  for (; n + 4 <= plain; n += 4) {
+    wait(n, Plain{});
+    before(now, n, Plain{});
+    step(now, 0, next, 1);
+    wait(n + 1, Plain{});
+    before(next, n + 1, Plain{});
+    step(next, 1, now, 2);
+    wait(n + 2, Plain{});
+    before(now, n + 2, Plain{});
+    step(now, 2, next, 3);
+    wait(n + 3, Plain{});
+    before(next, n + 3, Plain{});
+    step(next, 3, now, 0);
+  }
+  for (; n + 1 < np; ++n) {
+    wait(n, Any{});
+    before(now, n, Any{});
+    step(now, n & 3, next, (n + 1) & 3);
+#pragma unroll
+    for (int i = 0; i < N; ++i) now[i] = next[i];
+  }
+  wait(n, Any{});
+  before(now, n, Any{});
+  last(now, n & 3);
+}
+
+// Kept bits of up to MAX states in LDS, one word per 32: a mask is read once,
+// before the ring, so that no load of it waits behind a feed.
+struct XBits {
+  static constexpr int MAX = 32768, BYTES = MAX / 8;
+};
+
+template <class T, int DP, int WR, int WS, int DS, bool FWD>
 struct KeyStream {
   using I = Img<T, DP>;
   using E = typename T::elem;
-  static constexpr int NT = 64 * WR * WS * DS, SUB = KT / WS / 32, DH = DP / DS;
+  static constexpr int NT = 64 * WR * WS * DS, KT = 32 * WS, DH = DP / DS;
   static constexpr bool MEM = T::ES == 4;
-  static constexpr int TILE = MEM ? 0 : 2 * I::bytes(KT);
-  // two tiles (fp32: two exchanges of 8 KiB per wave), later the result
-  static constexpr int FED = MEM ? (DS > 1 ? 2 * 8192 * WR * WS * DS : 0) : 2 * TILE;
+  static constexpr int N = FWD ? 1 : 2, AHEAD = MEM ? 8 : 4;
+  static constexpr int TILE = MEM ? 0 : I::bytes(KT), SLOT = 2 * TILE;
+  // the ring and the mask's bits (fp32: two exchanges of 8 KiB per wave);
+  // later the result
+  static constexpr int BITS = 4 * SLOT;
+  static constexpr int FED = MEM ? (DS > 1 ? 2 * 8192 * WR * WS * DS : 0) : BITS + XBits::BYTES;
   static constexpr int STAT = 2 * 4 * 32 * WR * WS;
   static constexpr int OUT = x_store_bytes<T, DH, WR, WS>();
   static constexpr int OUT32 = x_store_bytes<XF32, DH, WR, WS>();
   static constexpr int LDS = x_max(x_max(FED, DS * OUT), STAT);
   static constexpr int LDS32 = x_max(x_max(FED, DS * OUT32), STAT);
 
-  // f(kept bits, K sources, V sources), one of each per piece of 32 states,
-  // for every tile; all waves of the block take part.
-  template <class F>
+  // before(sp, kept bits) and work(first, rest, sp, K, V, next, next K, next V)
+  // for the pieces of 32 states: sources of their operands; first, rest: which
+  // parts of a step to do (true_type).  All waves of the block take part.
+  template <class Before, class Work>
   static __device__ __forceinline__ void run(const XArgs& a, const XWork& w, int klo, int khi,
-                                             int ws, int ds, F f) {
+                                             int ws, int ds, Before before, Work work) {
+    using Yes = std::true_type;
+    using No = std::false_type;
     const int lane = threadIdx.x % 64;
     const uint8_t* mask = a.mask ? a.mask + w.b * a.mask_sb : nullptr;
     const E* K = x_key<E>(a.k, w.b, w.g, 0) + ds * DH;
     const E* V = x_key<E>(a.v, w.b, w.g, 0) + ds * DH;
     const uint32_t kst = (uint32_t)a.k.st * T::ES, vst = (uint32_t)a.v.st * T::ES;
     if constexpr (MEM) {
-      static_assert(SUB == 1, "one piece per wave");
       for (int t0 = klo; t0 < khi; t0 += KT) {
         const int k0 = t0 + 32 * ws, j = k0 + (lane & 31);
         const uint32_t kb = (uint32_t)__ballot(j < khi && (!mask || mask[j]));
@@ -495,65 +600,110 @@ struct KeyStream {
         MemSrc<DH> ks, vs;
         ks.begin(K + k0 * a.k.st, [&](int r) { return r * kst; }, kb, lane, a.D - ds * DH);
         vs.begin(V + k0 * a.v.st, [&](int r) { return r * vst; }, kb, lane, a.D - ds * DH);
-        const MemSrc<DH>*kp[1] = {&ks}, *vp[1] = {&vs};
-        const uint32_t kbs[1] = {kb};
-        f(kbs, kp, vp);
+        f32x16 sp[N];
+        work(Yes{}, No{}, sp, ks, vs, sp, ks, vs);
+        before(sp, kb);
+        work(No{}, Yes{}, sp, ks, vs, sp, ks, vs);
       }
     } else {
       static_assert(DS == 1, "whole rows");
-      constexpr uint32_t V0 = I::bytes(KT);
-      Feed<T, DP, KT, NT> fk, fv;
-      Keep<KT> kp;
-      fk.init([&](int r) { return r * kst; }, a.D);
-      fv.init([&](int r) { return r * vst; }, a.D);
-      __syncthreads();                   // the LDS may have been in use
-      for (uint32_t l0 = 0; l0 < 2 * TILE; l0 += TILE) {
-        fk.clear(l0);
-        fv.clear(l0 + V0);
+      for (int c = klo; c < khi; c += XBits::MAX)
+        part(a, mask, K, V, kst, vst, c, min(khi, c + XBits::MAX), ws, before, work);
+    }
+  }
+
+  template <class Before, class Work>
+  static __device__ __forceinline__ void part(const XArgs& a, const uint8_t* mask, const E* K,
+                                              const E* V, uint32_t kst, uint32_t vst, int klo,
+                                              int khi, int ws, Before before, Work work) {
+    using Yes = std::true_type;
+    using No = std::false_type;
+    const int lane = threadIdx.x % 64;
+    using F = Feed<T, DP, KT, NT>;
+    F fk, fv;
+    fk.init([&](int r) { return r * kst; }, a.D);
+    fv.init([&](int r) { return r * vst; }, a.D);
+    __syncthreads();                         // the LDS may have been in use
+    for (int i = 0; i < 4; ++i) {
+      fk.clear(i * SLOT);
+      fv.clear(i * SLOT + TILE);
+    }
+    const int np = (khi - klo + KT - 1) / KT, full = (khi - klo) / KT;
+    if (mask) {
+      for (int j = klo + (threadIdx.x & ~63); j < khi; j += NT) {
+        const uint64_t b = __ballot(j + lane < khi && mask[j + lane]);
+        if (lane < 2)
+          *(LDS_AS uint32_t*)(lds_base() + BITS + 4 * ((j - klo) / 32 + lane)) = b >> (32 * lane);
       }
-      auto start = [&](int k0, uint32_t l0) {
-        if (a.fast_k) {
-          fk.start(K + k0 * a.k.st, khi - k0, l0);
-          fv.start(V + k0 * a.v.st, khi - k0, l0 + V0);
-        } else {
-          fk.copy([&](int r) { return k0 + r < khi ? K + (k0 + r) * a.k.st : nullptr; }, a.D, l0);
-          fv.copy([&](int r) { return k0 + r < khi ? V + (k0 + r) * a.v.st : nullptr; }, a.D,
-                  l0 + V0);
-        }
-      };
-      // The tile behind the current one is fed while this one is worked on;
-      // its mask is loaded a tile earlier still, so that waiting for it does
-      // not wait for a feed.
-      kp.load(mask, klo, khi, lane);
-      if (klo < khi) start(klo, 0);
-      uint32_t l0 = 0;
-      for (int k0 = klo; k0 < khi; k0 += KT, l0 ^= TILE) {
-        ring_barrier<0>();
-        uint64_t keep[Keep<KT>::W];
-        const bool all = kp.bits(keep);
-        if (!all) {
-          auto gone = [&](int r) { return !((keep[KT <= 64 ? 0 : r >> 6] >> (r & 63)) & 1); };
-          fk.drop(gone, l0);
-          fv.drop(gone, l0 + V0);
+      __syncthreads();
+    }
+    // kept bits of 32 states from klo + 32 i on (any i), the same in all lanes
+    auto bits = [&](int i) X_INLINE -> uint32_t {
+      const int left = khi - klo - 32 * i;
+      if (left <= 0) return 0;
+      if (mask)
+        return __builtin_amdgcn_readfirstlane(
+            *(LDS_AS uint32_t*)(lds_base() + BITS + 4 * i));
+      return left >= 32 ? 0xffffffffu : (1u << left) - 1;
+    };
+    auto feed = [&](int n) X_INLINE {
+      const int k0 = klo + n * KT;
+      const uint32_t l0 = (n & 3) * SLOT;
+      if (n >= np) return;
+      if (!a.fast_k) {
+        fk.copy([&](int r) { return k0 + r < khi ? K + (k0 + r) * a.k.st : nullptr; }, a.D, l0);
+        fv.copy([&](int r) { return k0 + r < khi ? V + (k0 + r) * a.v.st : nullptr; }, a.D,
+                l0 + TILE);
+      } else {
+        fk.template start<false>(K + k0 * a.k.st, khi - k0, l0);
+        fv.template start<false>(V + k0 * a.v.st, khi - k0, l0 + TILE);
+      }
+    };
+    feed(0);
+    feed(1);
+    feed(2);
+    auto wait = [&](int n, auto plain) X_INLINE {
+      if constexpr (plain.value) {
+        ring_barrier<2 * F::N>();            // all but piece n + 2
+        const int k0 = klo + (n + 3) * KT;
+        const uint32_t l0 = ((n + 3) & 3) * SLOT;
+        fk.template start<true>(K + k0 * a.k.st, KT, l0);
+        fv.template start<true>(V + k0 * a.v.st, KT, l0 + TILE);
+      } else {
+        if (a.fast_k && n >= 0 && n + 2 < full)
+          ring_barrier<2 * F::N>();
+        else
+          ring_barrier<0>();
+        bool all = true;
+#pragma unroll
+        for (int i = 0; i < WS; ++i) all = all && bits((n + 1) * WS + i) == 0xffffffffu;
+        if (!all && n + 1 < np) {
+          auto gone = [&](int r) { return !((bits((n + 1) * WS + (r >> 5)) >> (r & 31)) & 1); };
+          fk.drop(gone, ((n + 1) & 3) * SLOT);
+          fv.drop(gone, ((n + 1) & 3) * SLOT + TILE);
           __syncthreads();
         }
-        kp.load(mask, k0 + KT, khi, lane);
-        if (k0 + KT < khi) start(k0 + KT, l0 ^ TILE);
-        uint32_t kbs[SUB];
-        LdsSrc<T, DP> ks[SUB], vs[SUB];
-        const LdsSrc<T, DP>*kq[SUB], *vq[SUB];
-#pragma unroll
-        for (int u = 0; u < SUB; ++u) {
-          const int r0 = (ws * SUB + u) * 32;
-          kbs[u] = (uint32_t)(keep[KT <= 64 ? 0 : r0 >> 6] >> (r0 & 63));
-          ks[u] = {l0 + I::bytes(r0), lane};
-          vs[u] = {l0 + V0 + I::bytes(r0), lane};
-          kq[u] = &ks[u];
-          vq[u] = &vs[u];
-        }
-        f(kbs, kq, vq);
+        if (n >= 0) feed(n + 3);
       }
-    }
+    };
+    const uint32_t mine = I::bytes(32) * ws;
+    auto src = [&](uint32_t at) { return LdsSrc<T, DP>{at + mine, lane}; };
+    auto K_ = [&](int slot) X_INLINE { return src(slot * SLOT); };
+    auto V_ = [&](int slot) X_INLINE { return src(slot * SLOT + TILE); };
+    x_pipe<N>(
+        np, a.fast_k && !mask ? full - 3 : 0, wait,
+        [&](f32x16 (&sp)[N], int s) X_INLINE {
+          work(Yes{}, No{}, sp, K_(s), V_(s), sp, K_(s), V_(s));
+        },
+        [&](f32x16 (&sp)[N], int n, auto plain) X_INLINE {
+          before(sp, plain.value ? 0xffffffffu : bits(n * WS + ws));
+        },
+        [&](f32x16 (&sp)[N], int s, f32x16 (&next)[N], int t) X_INLINE {
+          work(Yes{}, Yes{}, sp, K_(s), V_(s), next, K_(t), V_(t));
+        },
+        [&](f32x16 (&sp)[N], int s) X_INLINE {
+          work(No{}, Yes{}, sp, K_(s), V_(s), sp, K_(s), V_(s));
+        });
   }
 };
 
@@ -610,9 +760,9 @@ __device__ __forceinline__ void x_mask(f32x16& s, uint32_t kb, int h) {
 }
 
 // ------------------------------------------------------------------ forward ---
-template <class T, int DP, int WR, int WS, int DS, int KT, int OCC>
-__global__ __launch_bounds__(64 * WR * WS * DS, OCC) void xattn_fwd(const XArgs a) {
-  using S = KeyStream<T, DP, WR, WS, DS, KT>;
+template <class T, int DP, int WR, int WS, int DS, int OCC>
+__global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(const XArgs a) {
+  using S = KeyStream<T, DP, WR, WS, DS, true>;
   using I = Img<T, S::DH>;
   using E = typename T::elem;
   const XWork w = x_work(a);
@@ -623,13 +773,14 @@ __global__ __launch_bounds__(64 * WR * WS * DS, OCC) void xattn_fwd(const XArgs 
   const int row0 = w.tile * WR * 32, row = row0 + wr * 32 + lr;
   const int len = row0 < rows ? x_len(a.kv_lens, w.b, a.Tk) : 0;
   int klo, khi;
-  x_share(len, KT, a.splits, w.split, klo, khi);
+  x_share(len, S::KT, a.splits, w.split, klo, khi);
   const float c2 = a.scale * LOG2E_X;
 
   const int Dh = a.D - ds * S::DH;           // columns from this wave's first on
   Rows32<T, S::DH> qf;
   qf.load(row < rows ? x_row<E>(a.q, w.b, w.g, a.G, row) + ds * S::DH : nullptr, Dh, h);
-  f32x16 acc[S::DH / 32] = {};
+  constexpr int NB = S::DH / 32;
+  f32x16 acc[NB] = {};
   int turn = 0;
   // the reference that exponents are taken against, in the log2 domain:
   // exp(scale s - max) = 2^(c2 s - m).  It follows the running maximum only
@@ -637,22 +788,12 @@ __global__ __launch_bounds__(64 * WR * WS * DS, OCC) void xattn_fwd(const XArgs 
   // exact, probabilities stay below 2^8, and most tiles rescale nothing.
   float m = -INFINITY, l = 0.f;
 
-  S::run(a, w, klo, khi, ws, ds, [&](const uint32_t (&kb)[S::SUB], auto& ks, auto& vs) {
-    f32x16 s[S::SUB];
+  auto before = [&](f32x16 (&sp)[1], uint32_t kb) X_INLINE {
+    f32x16& s = sp[0];
+    x_mask(s, kb, h);
     float top = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < S::SUB; ++u) {
-      s[u] = f32x16{};
-#pragma unroll
-      for (int j = 0; j < I::NC; ++j) s[u] = T::mma(ks[u]->rm(j), qf[j], s[u]);
-    }
-    x_exchange<DS>(s, ws * WR + wr, ds, turn);
-#pragma unroll
-    for (int u = 0; u < S::SUB; ++u) {
-      x_mask(s[u], kb[u], h);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
-    }
+    for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
     top = xhalf_max(top) * c2;
     if (__any(top > m + 8.f || m == -INFINITY)) {
       const float mn = fmaxf(m, top);
@@ -662,21 +803,39 @@ __global__ __launch_bounds__(64 * WR * WS * DS, OCC) void xattn_fwd(const XArgs 
 #pragma unroll
       for (int db = 0; db < S::DH / 32; ++db) acc[db] *= al;
     }
+  };
+  S::run(a, w, klo, khi, ws, ds, before,
+         [&](auto first, auto rest, f32x16 (&sp)[1], const auto&, const auto& vs,
+             f32x16 (&next)[1], const auto& kn, const auto&) X_INLINE {
+    constexpr bool A = first.value, B = rest.value;
+    constexpr int RM = A ? I::NC : 0, TR = B ? I::NPF * NB : 0, PER = 16 / I::NC;
     const float mu = m == -INFINITY ? 0.f : m;        // no kept state so far
+    uint4 p[I::NPF];
+    auto probability = [&](int e) X_INLINE {
+      sp[0][e] = __builtin_amdgcn_exp2f(fmaf(sp[0][e], c2, -mu));
+      l += sp[0][e];
+    };
+    if constexpr (A) next[0] = f32x16{};
+    x_step<RM, TR, S::AHEAD>(
+        [&](int i) X_INLINE { return kn.rm(i); },
+        [&](int i, uint4 f) X_INLINE { next[0] = T::mma(f, qf[i], next[0]); },
+        [&](int i) X_INLINE {
+          if constexpr (B)
 #pragma unroll
-    for (int u = 0; u < S::SUB; ++u) {
+            for (int e = i * PER; e < (i + 1) * PER; ++e) probability(e);
+        },
+        [&]() X_INLINE {
+          if constexpr (B) {
+            if constexpr (!A)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        s[u][e] = __builtin_amdgcn_exp2f(fmaf(s[u][e], c2, -mu));
-        l += s[u][e];
-      }
+              for (int e = 0; e < 16; ++e) probability(e);
 #pragma unroll
-      for (int c = 0; c < I::NPF; ++c) {
-        const uint4 p = I::pack(s[u], c);
-#pragma unroll
-        for (int db = 0; db < S::DH / 32; ++db) acc[db] = T::mma(vs[u]->tr(c, db), p, acc[db]);
-      }
-    }
+            for (int c = 0; c < I::NPF; ++c) p[c] = I::pack(sp[0], c);
+          }
+        },
+        [&](int i) X_INLINE { return vs.tr(i / NB, i % NB); },
+        [&](int i, uint4 f) X_INLINE { acc[i % NB] = T::mma(f, p[i / NB], acc[i % NB]); });
+    if constexpr (A && !B) x_exchange<DS>(next, ws * WR + wr, ds, turn);
   });
   l = xhalf_sum(l);
 
@@ -763,9 +922,9 @@ __device__ __forceinline__ float x_down(float amax) {
 
 // dQ of WR * 32 rows, streaming K and V; also delta (and the rows' |dO|) for
 // xattn_dkv, which runs after it.
-template <class T, int DP, int WR, int WS, int DS, int KT, int OCC>
-__global__ __launch_bounds__(64 * WR * WS * DS, OCC) void xattn_dq(const XArgs a) {
-  using S = KeyStream<T, DP, WR, WS, DS, KT>;
+template <class T, int DP, int WR, int WS, int DS, int OCC>
+__global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(const XArgs a) {
+  using S = KeyStream<T, DP, WR, WS, DS, false>;
   using I = Img<T, S::DH>;
   using E = typename T::elem;
   const XWork w = x_work(a);
@@ -776,7 +935,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS, OCC) void xattn_dq(const XArgs a
   const int row0 = w.tile * WR * 32, row = row0 + wr * 32 + lr;
   const int len = row0 < rows ? x_len(a.kv_lens, w.b, a.Tk) : 0;
   int klo, khi;
-  x_share(len, KT, a.splits, w.split, klo, khi);
+  x_share(len, S::KT, a.splits, w.split, klo, khi);
   const float c2 = a.scale * LOG2E_X;
   const long long at = (long long)w.bh * a.R;
 
@@ -815,33 +974,53 @@ __global__ __launch_bounds__(64 * WR * WS * DS, OCC) void xattn_dq(const XArgs a
   const float down = x_down<T>(amax);
   int turn = 0;
 
-  // P of a piece in sp[0], dP in sp[1]
-  auto scores = [&](f32x16 (&sp)[2], uint32_t kb, const auto* ks, const auto* vs) {
-    sp[0] = sp[1] = f32x16{};
+  auto masked = [&](f32x16 (&sp)[2], uint32_t kb) X_INLINE { x_mask(sp[0], kb, h); };
+  constexpr int NB = S::DH / 32;
+  f32x16 acc[NB] = {};
+  // the scores of a piece in sp[0], dP in sp[1]; element(sp, e): their vector work
+  auto run = [&](auto products, auto element) X_INLINE {
+    S::run(a, w, klo, khi, ws, ds, masked,
+           [&](auto first, auto rest, f32x16 (&sp)[2], const auto& ks, const auto&,
+               f32x16 (&next)[2], const auto& kn, const auto& vn) X_INLINE {
+      constexpr bool A = first.value, B = rest.value, P = decltype(products)::value;
+      constexpr int RM = A ? 2 * I::NC : 0, TR = B && P ? I::NPF * NB : 0;
+      uint4 p[I::NPF];
+      if constexpr (A) next[0] = next[1] = f32x16{};
+      x_step<RM, TR, S::AHEAD>(
+          [&](int i) X_INLINE { return i & 1 ? vn.rm(i / 2) : kn.rm(i / 2); },
+          [&](int i, uint4 f) X_INLINE {
+            next[i & 1] = T::mma(f, i & 1 ? df[i / 2] : qf[i / 2], next[i & 1]);
+          },
+          [&](int i) X_INLINE {
+            if constexpr (B)
 #pragma unroll
-    for (int j = 0; j < I::NC; ++j) {
-      sp[0] = T::mma(ks->rm(j), qf[j], sp[0]);
-      sp[1] = T::mma(vs->rm(j), df[j], sp[1]);
-    }
-    x_exchange<DS>(sp, ws * WR + wr, ds, turn);
-    x_mask(sp[0], kb, h);
+              for (int e = 0; e < 16; ++e)
+                if (e * RM / 16 == i) element(sp, e);
+          },
+          [&]() X_INLINE {
+            if constexpr (B && !A)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) sp[0][e] = __builtin_amdgcn_exp2f(fmaf(sp[0][e], c2, -L));
+              for (int e = 0; e < 16; ++e) element(sp, e);
+            if constexpr (TR > 0)
+#pragma unroll
+              for (int c = 0; c < I::NPF; ++c) p[c] = I::pack(sp[0], c);
+          },
+          [&](int i) X_INLINE { return ks.tr(i / NB, i % NB); },
+          [&](int i, uint4 f) X_INLINE { acc[i % NB] = T::mma(f, p[i / NB], acc[i % NB]); });
+      if constexpr (A && !B) x_exchange<DS>(next, ws * WR + wr, ds, turn);
+    });
   };
-  // With one tile of states, delta = sum P dP is summed from the products
-  // themselves: dO . O carries the rounding of O to the type, which few states
-  // do not average out (dQ was 1.53 times as far off as one rounding at 32
-  // states, against 1.42 times so).
-  if (T::ES == 2 && a.Tk <= KT) {
+  auto probability = [&](float s) X_INLINE {
+    return __builtin_amdgcn_exp2f(fmaf(s, c2, -L));
+  };
+  // With few states, delta = sum P dP is summed from the products themselves:
+  // dO . O carries the rounding of O to the type, which few states do not
+  // average out (dQ was 1.53 times as far off as one rounding at 32 states,
+  // against 1.42 times so).
+  if (T::ES == 2 && a.Tk <= 64 && a.splits == 1) {
     float sum = 0.f;
-    S::run(a, w, klo, khi, ws, ds, [&](const uint32_t (&kb)[S::SUB], auto& ks, auto& vs) {
-#pragma unroll
-      for (int u = 0; u < S::SUB; ++u) {
-        f32x16 sp[2];
-        scores(sp, kb[u], ks[u], vs[u]);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) sum = fmaf(sp[0][e], sp[1][e], sum);
-      }
+    run(std::false_type{}, [&](f32x16 (&sp)[2], int e) X_INLINE {
+      sum = fmaf(probability(sp[0][e]), sp[1][e], sum);
     });
     sum = xhalf_sum(sum);
     if constexpr (WS > 1) {
@@ -857,24 +1036,9 @@ __global__ __launch_bounds__(64 * WR * WS * DS, OCC) void xattn_dq(const XArgs a
     a.delta[at + row] = delta;
     if (a.amax) a.amax[at + row] = amax;
   }
-  f32x16 acc[S::DH / 32] = {};
-  S::run(a, w, klo, khi, ws, ds, [&](const uint32_t (&kb)[S::SUB], auto& ks, auto& vs) {
-#pragma unroll
-    for (int u = 0; u < S::SUB; ++u) {
-      f32x16 sp[2];
-      scores(sp, kb[u], ks[u], vs[u]);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        sp[0][e] *= sp[1][e] - delta;
-        if constexpr (std::is_same<T, XF16>::value) sp[0][e] *= down;
-      }
-#pragma unroll
-      for (int c = 0; c < I::NPF; ++c) {
-        const uint4 p = I::pack(sp[0], c);
-#pragma unroll
-        for (int db = 0; db < S::DH / 32; ++db) acc[db] = T::mma(ks[u]->tr(c, db), p, acc[db]);
-      }
-    }
+  run(std::true_type{}, [&](f32x16 (&sp)[2], int e) X_INLINE {
+    sp[0][e] = probability(sp[0][e]) * (sp[1][e] - delta);
+    if constexpr (std::is_same<T, XF16>::value) sp[0][e] *= down;
   });
   const float mul = a.scale / down;
   const bool none = L == INFINITY;
@@ -891,27 +1055,27 @@ __global__ __launch_bounds__(64 * WR * WS * DS, OCC) void xattn_dq(const XArgs a
   }
 }
 
-// dK and dV of WC * 32 states, streaming Q and dO over RT rows at a time; WS
+// dK and dV of WC * 32 states, streaming Q and dO, 32 WS rows at a time; WS
 // waves share the states and take different rows, DS waves the columns of the
 // results: of fp32 as above, of 16-bit types with 256 columns because both
 // accumulators are too large for one wave's registers (each of the two forms
 // all of the scores, 6 products where 4 would do).
-template <class T, int DP, int WC, int WS, int DS, int RT>
+template <class T, int DP, int WC, int WS, int DS>
 struct DkvCfg {
-  static constexpr int NT = 64 * WC * WS * DS;
-  static constexpr int SUB = RT / WS / 32;
+  static constexpr int NT = 64 * WC * WS * DS, RT = 32 * WS, AHEAD = T::ES == 4 ? 8 : 4;
   static constexpr bool MEM = T::ES == 4;
   static constexpr int TILE = MEM ? 0 : 2 * Img<T, DP>::bytes(RT) + 8 * RT;   // Q, dO, L, delta
-  static constexpr int FED = MEM ? (DS > 1 ? 2 * 8192 * WC * WS * DS : 0) : 2 * TILE;
+  static constexpr int FED = MEM ? (DS > 1 ? 2 * 8192 * WC * WS * DS : 0) : 4 * TILE;
   static constexpr int OUT = x_store_bytes<T, DP / DS, WC, WS>();
   static constexpr int OUT32 = x_store_bytes<XF32, DP / DS, WC, WS>();
   static constexpr int LDS = x_max(x_max(FED, DS * OUT), 64);
   static constexpr int LDS32 = x_max(LDS, DS * OUT32);
 };
 
-template <class T, int DP, int WC, int WS, int DS, int RT, int OCC>
-__global__ __launch_bounds__(64 * WC * WS * DS, OCC) void xattn_dkv(const XArgs a) {
-  using C = DkvCfg<T, DP, WC, WS, DS, RT>;
+template <class T, int DP, int WC, int WS, int DS, int OCC>
+__global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(const XArgs a) {
+  using C = DkvCfg<T, DP, WC, WS, DS>;
+  constexpr int RT = C::RT;
   // operands: a wave's own columns (fp32) or all
   constexpr int DH = DP / DS, NB = DH / 32, DO = C::MEM ? DH : DP;
   using I = Img<T, DO>;
@@ -948,38 +1112,65 @@ __global__ __launch_bounds__(64 * WC * WS * DS, OCC) void xattn_dkv(const XArgs 
   f32x16 dk[NB] = {}, dv[NB] = {};
   int turn = 0;
 
-  // one piece of 32 rows: L and delta of row acc_row(4 k + e, h) in element e
-  // of stat(k)
-  auto piece = [&](const auto& qs, const auto& os, auto lse, auto del) {
-    f32x16 sp[2] = {};
-#pragma unroll
-    for (int j = 0; j < I::NC; ++j) {
-      sp[0] = T::mma(qs.rm(j), kf[j], sp[0]);
-      sp[1] = T::mma(os.rm(j), vf[j], sp[1]);
-    }
-    if constexpr (C::MEM) x_exchange<DS>(sp, ws * WC + wc, ds, turn);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const f32x4 L = lse(k), t = del(k);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = 4 * k + e;
-        sp[0][i] = __builtin_amdgcn_exp2f(fmaf(sp[0][i], c2, -L[e]));
-        sp[1][i] = sp[0][i] * (sp[1][i] - t[e]);
-        if constexpr (std::is_same<T, XF16>::value) sp[1][i] *= down;
-      }
-    }
+  // A step as x_step runs it: scores and dP of `next` beside the rest of sp, a
+  // piece of 32 rows; lse(k), del(k): L and delta of its rows acc_row(4 k + e, h)
+  auto work = [&](auto first, auto rest, f32x16 (&sp)[2], const auto& qs, const auto& os, auto lse,
+                  auto del, f32x16 (&next)[2], const auto& qn, const auto& on) X_INLINE {
+    constexpr bool A = first.value, B = rest.value;
+    constexpr int RM = A ? 2 * I::NC : 0, TR = B ? 2 * I::NPF * NB : 0;
     const int b0 = C::MEM ? 0 : ds * NB;
+    f32x4 L[4], t[4];
+    if constexpr (B)
 #pragma unroll
-    for (int c = 0; c < I::NPF; ++c) {
-      const uint4 p = I::pack(sp[0], c), g = I::pack(sp[1], c);
-#pragma unroll
-      for (int db = 0; db < NB; ++db) {
-        dv[db] = T::mma(os.tr(c, b0 + db), p, dv[db]);
-        dk[db] = T::mma(qs.tr(c, b0 + db), g, dk[db]);
+      for (int k = 0; k < 4; ++k) {
+        L[k] = lse(k);
+        t[k] = del(k);
       }
-    }
+    uint4 p[I::NPF], g[I::NPF];
+    auto element = [&](int i) X_INLINE {
+      sp[0][i] = __builtin_amdgcn_exp2f(fmaf(sp[0][i], c2, -L[i / 4][i % 4]));
+      sp[1][i] = sp[0][i] * (sp[1][i] - t[i / 4][i % 4]);
+      if constexpr (std::is_same<T, XF16>::value) sp[1][i] *= down;
+    };
+    if constexpr (A) next[0] = next[1] = f32x16{};
+    x_step<RM, TR, C::AHEAD>(
+        [&](int i) X_INLINE { return i & 1 ? on.rm(i / 2) : qn.rm(i / 2); },
+        [&](int i, uint4 f) X_INLINE {
+          next[i & 1] = T::mma(f, i & 1 ? vf[i / 2] : kf[i / 2], next[i & 1]);
+        },
+        [&](int i) X_INLINE {
+          if constexpr (B)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (e * RM / 16 == i) element(e);
+        },
+        [&]() X_INLINE {
+          if constexpr (B) {
+            if constexpr (!A)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) element(e);
+#pragma unroll
+            for (int c = 0; c < I::NPF; ++c) {
+              p[c] = I::pack(sp[0], c);
+              g[c] = I::pack(sp[1], c);
+            }
+          }
+        },
+        [&](int i) X_INLINE {
+          const int c = i / 2 / NB, db = i / 2 % NB;
+          return i & 1 ? qs.tr(c, b0 + db) : os.tr(c, b0 + db);
+        },
+        [&](int i, uint4 f) X_INLINE {
+          const int c = i / 2 / NB, db = i / 2 % NB;
+          if (i & 1)
+            dk[db] = T::mma(f, g[c], dk[db]);
+          else
+            dv[db] = T::mma(f, p[c], dv[db]);
+        });
+    if constexpr (C::MEM && A && !B) x_exchange<DS>(next, ws * WC + wc, ds, turn);
   };
+  using Yes = std::true_type;
+  using No = std::false_type;
   // byte offset of row i of a tile that begins with a token's first head
   auto in_tile = [&](const XView& v) {
     const uint32_t st = (uint32_t)v.st * T::ES, sh = (uint32_t)v.sh * T::ES;
@@ -1013,64 +1204,107 @@ __global__ __launch_bounds__(64 * WC * WS * DS, OCC) void xattn_dkv(const XArgs 
           return v;
         };
       };
-      piece(qs, os, stat(a.lse, INFINITY), stat(a.delta, 0.f));
+      f32x16 sp[2];
+      const auto lse = stat(a.lse, INFINITY), del = stat(a.delta, 0.f);
+      work(Yes{}, No{}, sp, qs, os, lse, del, sp, qs, os);
+      work(No{}, Yes{}, sp, qs, os, lse, del, sp, qs, os);
     }
   } else {
     constexpr uint32_t D0 = I::bytes(RT), L0 = 2 * D0, T0 = L0 + 4 * RT;
-    Feed<T, DP, RT, C::NT> fq, fd;
+    using F = Feed<T, DP, RT, C::NT>;
+    constexpr int STATS = (RT + 63) / 64;             // instructions for L, delta each
+    F fq, fd;
     fq.init(in_tile(a.q), a.D);
     fd.init(in_tile(a.dout), a.D);
-    for (uint32_t l0 = 0; l0 < 2 * C::TILE; l0 += C::TILE) {
-      fq.clear(l0);
-      fd.clear(l0 + D0);
+    __syncthreads();
+    for (int i = 0; i < 4; ++i) {
+      fq.clear(i * C::TILE);
+      fd.clear(i * C::TILE + D0);
     }
-    float fl = INFINITY, ft = 0.f;
-    auto stats = [&](int r0) {
-      const int r = r0 + threadIdx.x;
-      const bool in = threadIdx.x < RT && r < rhi;
-      fl = in ? a.lse[at + r] : INFINITY;
-      ft = in ? a.delta[at + r] : 0.f;
+    const int np = (rhi - rlo + RT - 1) / RT, full = (rhi - rlo) / RT;
+    // L and delta of a tile; every wave fetches them (the same values to the
+    // same places), so that all waves count the same instructions
+    auto stats = [&](int r0, uint32_t l0) X_INLINE {
+#pragma unroll
+      for (int i = 0; i < STATS; ++i)
+        if (64 * i + lane < RT && r0 + 64 * i + lane < rhi) {
+          dma4(a.lse + at + r0, 4 * (64 * i + lane), l0 + L0 + 256 * i);
+          dma4(a.delta + at + r0, 4 * (64 * i + lane), l0 + T0 + 256 * i);
+        }
     };
-    auto start = [&](int r0, uint32_t l0) {
-      if (threadIdx.x < RT) {
-        lds_stf(l0 + L0 + 4 * threadIdx.x, fl);
-        lds_stf(l0 + T0 + 4 * threadIdx.x, ft);
-      }
-      stats(r0 + RT);       // of the tile after: waiting for it then waits for no feed
-      if (a.fast_q) {       // G divides RT: a tile begins with a token's first head
-        fq.start(x_row<E>(a.q, w.b, w.g, a.G, r0), rhi - r0, l0);
-        fd.start(x_row<E>(a.dout, w.b, w.g, a.G, r0), rhi - r0, l0 + D0);
-      } else {
+    // a tile's first row, where G, a power of two, divides RT
+    const int sh = 31 - __builtin_clz(a.G);
+    auto first = [&](const XView& v, int r0) -> const E* {
+      return x_row<E>(v, w.b, w.g, a.G, 0) + (long long)(r0 >> sh) * v.st;
+    };
+    auto feed = [&](int n) X_INLINE {
+      const int r0 = rlo + n * RT;
+      const uint32_t l0 = (n & 3) * C::TILE;
+      if (n >= np) return;
+      stats(r0, l0);
+      if (!a.fast_q) {
         fq.copy([&](int r) {
           return r0 + r < rhi ? x_row<E>(a.q, w.b, w.g, a.G, r0 + r) : nullptr; }, a.D, l0);
         fd.copy([&](int r) {
           return r0 + r < rhi ? x_row<E>(a.dout, w.b, w.g, a.G, r0 + r) : nullptr; }, a.D, l0 + D0);
+      } else {
+        fq.template start<false>(first(a.q, r0), rhi - r0, l0);
+        fd.template start<false>(first(a.dout, r0), rhi - r0, l0 + D0);
       }
     };
-    stats(rlo);
-    if (rlo < rhi) start(rlo, 0);
-    uint32_t l0 = 0;
-    for (int t0 = rlo; t0 < rhi; t0 += RT, l0 ^= C::TILE) {
-      ring_barrier<0>();
-      if (t0 + RT > rhi) {
-        auto gone = [&](int r) { return t0 + r >= rhi; };
-        fq.drop(gone, l0);
-        fd.drop(gone, l0 + D0);
-        __syncthreads();
+    feed(0);
+    feed(1);
+    feed(2);
+    auto wait = [&](int n, auto plain) X_INLINE {
+      if constexpr (plain.value) {
+        ring_barrier<2 * F::N + 2 * STATS>();
+        const int r0 = rlo + (n + 3) * RT;
+        const uint32_t l0 = ((n + 3) & 3) * C::TILE;
+        stats(r0, l0);
+        fq.template start<true>(first(a.q, r0), RT, l0);
+        fd.template start<true>(first(a.dout, r0), RT, l0 + D0);
+      } else {
+        if (a.fast_q && n >= 0 && n + 2 < full)
+          ring_barrier<2 * F::N + 2 * STATS>();
+        else
+          ring_barrier<0>();
+        const int t0 = rlo + (n + 1) * RT;
+        if (t0 < rhi && t0 + RT > rhi) {
+          auto gone = [&](int r) { return t0 + r >= rhi; };
+          const uint32_t l0 = ((n + 1) & 3) * C::TILE;
+          fq.drop(gone, l0);
+          fd.drop(gone, l0 + D0);
+          if (threadIdx.x < RT && gone(threadIdx.x)) {
+            lds_stf(l0 + L0 + 4 * threadIdx.x, INFINITY);
+            lds_stf(l0 + T0 + 4 * threadIdx.x, 0.f);
+          }
+          __syncthreads();
+        }
+        if (n >= 0) feed(n + 3);
       }
-      if (t0 + RT < rhi) start(t0 + RT, l0 ^ C::TILE);
-#pragma unroll
-      for (int u = 0; u < C::SUB; ++u) {
-        const int r0 = (ws * C::SUB + u) * 32;
-        const LdsSrc<T, DP> qs{l0 + I::bytes(r0), lane}, os{l0 + D0 + I::bytes(r0), lane};
-        auto stat = [&](uint32_t base) {
-          return [=](int k) {
-            return __builtin_bit_cast(f32x4, lds_ld16(base + 4 * (r0 + 8 * k + 4 * h)));
-          };
-        };
-        piece(qs, os, stat(l0 + L0), stat(l0 + T0));
-      }
-    }
+    };
+    const uint32_t mine = I::bytes(32) * ws;
+    auto src = [&](uint32_t l0) { return LdsSrc<T, DP>{l0 + mine, lane}; };
+    auto stat = [&](int slot, uint32_t what) X_INLINE {
+      return [=](int k) X_INLINE {
+        return __builtin_bit_cast(
+            f32x4, lds_ld16(slot * C::TILE + what + 4 * (32 * ws + 8 * k + 4 * h)));
+      };
+    };
+    auto Q_ = [&](int slot) X_INLINE { return src(slot * C::TILE); };
+    auto O_ = [&](int slot) X_INLINE { return src(slot * C::TILE + D0); };
+    x_pipe<2>(
+        np, a.fast_q ? full - 3 : 0, wait,
+        [&](f32x16 (&sp)[2], int s) X_INLINE {
+          work(Yes{}, No{}, sp, Q_(s), O_(s), stat(s, L0), stat(s, T0), sp, Q_(s), O_(s));
+        },
+        [](f32x16 (&)[2], int, auto) {},
+        [&](f32x16 (&sp)[2], int s, f32x16 (&next)[2], int t) X_INLINE {
+          work(Yes{}, Yes{}, sp, Q_(s), O_(s), stat(s, L0), stat(s, T0), next, Q_(t), O_(t));
+        },
+        [&](f32x16 (&sp)[2], int s) X_INLINE {
+          work(No{}, Yes{}, sp, Q_(s), O_(s), stat(s, L0), stat(s, T0), sp, Q_(s), O_(s));
+        });
   }
   const int tid = threadIdx.x % (64 * WC * WS), Dh = min(a.D - ds * DH, DH);
   const float mul = a.scale / down;
@@ -1125,9 +1359,9 @@ struct XPlan {
 constexpr int x_columns(int type, int what, int dp) {
   return type == 1 ? dp / 64 : what == X_DKV && dp == 256 ? 2 : 1;
 }
-// least waves along the rows
+// Least waves that own rows (states): the rings of fewer would pass the LDS.
 constexpr int x_least(int type, int what, int dp) {
-  return type != 1 && what != X_DKV && dp == 256 ? 2 : 1;
+  return type == 1 || dp <= 64 ? 1 : dp == 128 || what == X_DKV ? 2 : 4;
 }
 // The split of one kernel's work.  `own` rows (dK, dV: states) belong to the
 // waves, the others are streamed.  A block's four waves (or those that the
@@ -1162,36 +1396,36 @@ int x_go(K kernel, const XArgs& a, int lds, int nt, void* stream) {
   return (int)hipGetLastError();
 }
 
-template <class T, int DP, int W>
-int x_rows(const XArgs& a, int what, void* stream) {
-  // fp32 takes one piece of 32 states per wave; 16-bit tiles hold 64 states,
-  // 128 where four waves share them (of 256 columns two such tiles would pass
-  // the LDS: x_least)
+template <class T, int DP, int W, bool FWD>
+int x_rows(const XArgs& a, void* stream) {
   constexpr int DS = x_columns(T::TYPE, X_FWD, DP), WS = 4 / DS / W;
-  constexpr int KT = T::ES == 4 ? 32 * WS : W == 1 ? 128 : 64;
-  constexpr int OCC = T::ES == 4 ? 2 : DP <= 128 && W > 1 ? 2 : 1;
-  using S = KeyStream<T, DP, W, WS, DS, KT>;
+  constexpr int OCC = T::ES == 4 || DP * (4 / W) <= 128 ? 2 : 1;        // rings of 64 KiB
+  using S = KeyStream<T, DP, W, WS, DS, FWD>;
   const int lds = a.splits > 1 ? S::LDS32 : S::LDS;
-  return what == X_FWD ? x_go(xattn_fwd<T, DP, W, WS, DS, KT, OCC>, a, lds, S::NT, stream)
-                       : x_go(xattn_dq<T, DP, W, WS, DS, KT, OCC>, a, lds, S::NT, stream);
+  if constexpr (FWD)
+    return x_go(xattn_fwd<T, DP, W, WS, DS, OCC>, a, lds, S::NT, stream);
+  else
+    return x_go(xattn_dq<T, DP, W, WS, DS, OCC>, a, lds, S::NT, stream);
 }
 template <class T, int DP, int W>
 int x_states(const XArgs& a, void* stream) {
   constexpr int DS = x_columns(T::TYPE, X_DKV, DP), WS = 4 / DS / W;
-  using C = DkvCfg<T, DP, W, WS, DS, 32 * WS>;
-  return x_go(xattn_dkv<T, DP, W, WS, DS, 32 * WS, 1>, a, a.splits > 1 ? C::LDS32 : C::LDS, C::NT,
-              stream);
+  using C = DkvCfg<T, DP, W, WS, DS>;
+  return x_go(xattn_dkv<T, DP, W, WS, DS, 1>, a, a.splits > 1 ? C::LDS32 : C::LDS, C::NT, stream);
 }
 template <class T, int DP, int W>
 int x_waves(const XArgs& a, int waves, int what, void* stream) {
   if constexpr (W > 1)
     if (waves < W) return x_waves<T, DP, W / 2>(a, waves, what, stream);
-  if (what == X_DKV) {
-    if constexpr (W * x_columns(T::TYPE, X_DKV, DP) <= 4) return x_states<T, DP, W>(a, stream);
-  } else {
-    if constexpr (W * x_columns(T::TYPE, X_FWD, DP) <= 4 && W >= x_least(T::TYPE, X_FWD, DP))
-      return x_rows<T, DP, W>(a, what, stream);
-  }
+  constexpr auto takes = [](int k) {
+    return W * x_columns(T::TYPE, k, DP) <= 4 && W >= x_least(T::TYPE, k, DP);
+  };
+  if constexpr (takes(X_FWD))
+    if (what == X_FWD) return x_rows<T, DP, W, true>(a, stream);
+  if constexpr (takes(X_DQ))
+    if (what == X_DQ) return x_rows<T, DP, W, false>(a, stream);
+  if constexpr (takes(X_DKV))
+    if (what == X_DKV) return x_states<T, DP, W>(a, stream);
   return 1001;
 }
 
