@@ -14,9 +14,11 @@
 // it in 64-bit integers drops whole turns exactly, for any position; the
 // fraction's own rounding makes the angle off by at most pos 2^-65 turns.
 //
-// Bound by memory: x is read once and y written once.  16 bytes per lane and
-// load; a wave takes one token, LPR lanes per head, so the sines of a lane's
-// pairs are formed once and serve all heads of the token.
+// Bound by memory: x is read once and y written once, 16 bytes per lane and
+// load, LPR lanes per head.  A wave takes one token, or as many as fill it
+// where heads are few; its lanes form the sines of the tokens' pairs once, each
+// another one, and share them through LDS (formed by each lane for itself,
+// they took more vector instructions than all the rest).
 #include "tgfr_common.h"
 
 using namespace tgfr;
@@ -34,13 +36,15 @@ struct NPart {
   const void* pos;      // positions; NULL: 0 .. T - 1 on every axis
   long long pb, pt, pa;
   int B, T, H;
-  int blocks;           // backward: blocks of this part
+  int lg;               // 2^lg >= min(H, 64 / LPR) heads of a token side by side
+  int blocks;           // of this part
 };
 struct NArgs {
   NPart p[2];
   const unsigned long long* turn;   // [R / 2]
   float* part;          // backward: [blocks][D] partial dw
-  int D, R, per, interleaved, pos32, heads;   // heads: per wave and unit
+  int D, R, per, interleaved, pos32;
+  int many;             // a unit takes all heads of its tokens
   float eps;
 };
 
@@ -151,170 +155,193 @@ __device__ __forceinline__ void n_store(const NArgs& a, void* base, int p0,
   }
 }
 
-// sines of a lane's pairs at one token
-template <int V>
-__device__ __forceinline__ void n_angles(const NArgs& a, const NPart& q, int b, int t, int p0,
-                                         const unsigned long long (&turn)[V], float (&cs)[V],
-                                         float (&sn)[V]) {
-  long long last = 0;
-  int axis = -1;
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    cs[i] = 1.f;
-    sn[i] = 0.f;
-    if (p0 + i < a.R / 2) {
-      const int ax = (p0 + i) / a.per;
-      if (ax != axis) {
-        axis = ax;
-        last = t;
-        if (q.pos) {
-          const long long at = b * q.pb + t * q.pt + ax * q.pa;
-          last = a.pos32 ? ((const int*)q.pos)[at] : ((const long long*)q.pos)[at];
-        }
-      }
-      const unsigned long long f = (unsigned long long)last * turn[i];
-      // signed fraction of a turn, [-1/2, 1/2)
-      const float turns = fmaf((float)(uint32_t)f, 0x1p-64f, (float)(int32_t)(f >> 32) * 0x1p-32f);
-      sincospif(2.f * turns, &sn[i], &cs[i]);
-    }
-  }
-}
-
 template <int LPR>
 __device__ __forceinline__ float n_sum(float v) {
-#pragma unroll
-  for (int m = LPR / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m);
-  return v;
+  if constexpr (LPR >= 64) v = xhalf_sum(v);
+  if constexpr (LPR >= 32) v = x16_sum(v);
+  if constexpr (LPR >= 16) v += dpp<0x140>(v);
+  if constexpr (LPR >= 8) v += dpp<0x141>(v);
+  v += dpp<0xB1>(v);
+  return v + dpp<0x4E>(v);
 }
 
-// One unit of a wave: a token and `heads` of its heads, IT times 64 / LPR at
-// once.
+// A wave's unit: 64 / LPR >> lg tokens, and 2^lg of their heads at once.
+template <int V, int LPR>
+struct Unit {
+  static constexpr int HPW = 64 / LPR;
+  int h0, h1, step;          // this lane's heads: h0, h0 + step, ... below h1
+  int b, t;                  // its token (valid: it has one)
+  bool valid;
+
+  static __device__ __forceinline__ long long count(const NArgs& a, const NPart& q) {
+    const long long tokens = (long long)q.B * q.T, at_once = HPW >> q.lg;
+    return (tokens + at_once - 1) / at_once * (a.many ? 1 : (q.H + (1 << q.lg) - 1) >> q.lg);
+  }
+  static __device__ __forceinline__ void token(const NPart& q, int id, int& b, int& t) {
+    b = (unsigned)id / (unsigned)q.T;
+    t = id - b * q.T;
+  }
+  // sc: LDS of the wave, V * 64 pairs (sine, cosine)
+  __device__ __forceinline__ Unit(const NArgs& a, const NPart& q, long long unit, float2* sc) {
+    const int lane = threadIdx.x % 64, g = lane / LPR;
+    const int hu = a.many ? 1 : (q.H + (1 << q.lg) - 1) >> q.lg;
+    const int tg = hu == 1 ? (int)unit : (int)(unit / hu), hc = (int)(unit - (long long)tg * hu);
+    const int tokens = q.B * q.T, first = tg * (HPW >> q.lg);
+    step = 1 << q.lg;
+    h0 = hc * step + (g & (step - 1));
+    h1 = a.many ? q.H : min(q.H, (hc + 1) * step);
+    valid = first + (g >> q.lg) < tokens;
+    token(q, min(first + (g >> q.lg), tokens - 1), b, t);
+    // Sines: 64 / (tokens of the wave) lanes per token, pair after pair.
+    const int per = LPR << q.lg;                      // lanes per token
+    int sb, st;
+    token(q, min(first + lane / per, tokens - 1), sb, st);
+    for (int p = lane & (per - 1); p < LPR * V; p += per) {
+      float2 v = make_float2(0.f, 1.f);
+      if (p < a.R / 2) {
+        long long at = st;
+        if (q.pos) {
+          const long long i = sb * q.pb + st * q.pt + (a.per == a.R / 2 ? 0 : p / a.per) * q.pa;
+          at = a.pos32 ? ((const int*)q.pos)[i] : ((const long long*)q.pos)[i];
+        }
+        const unsigned long long f = (unsigned long long)at * a.turn[p];
+        // signed fraction of a turn, [-1/2, 1/2)
+        const float turns =
+            fmaf((float)(uint32_t)f, 0x1p-64f, (float)(int32_t)(f >> 32) * 0x1p-32f);
+        sincospif(2.f * turns, &v.x, &v.y);
+      }
+      sc[lane / per * (LPR * V) + p] = v;
+    }
+    __builtin_amdgcn_wave_barrier();                  // (one wave's LDS is in order)
+  }
+  __device__ __forceinline__ void sines(const NPart& q, const float2* sc, float (&sn)[V],
+                                        float (&cs)[V]) const {
+    const int lane = threadIdx.x % 64, c = lane % LPR, g = lane / LPR;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float2 v = sc[(g >> q.lg) * (LPR * V) + c * V + i];
+      sn[i] = v.x;
+      cs[i] = v.y;
+    }
+  }
+};
+
+// this block's part, and its place among that part's blocks
+__device__ __forceinline__ int n_part(const NArgs& a, int& blk) {
+  const int k = (int)blockIdx.x >= a.p[0].blocks;
+  blk = k ? blockIdx.x - a.p[0].blocks : blockIdx.x;
+  return k;
+}
+
 template <int KI, int KO, int V, int LPR, bool CH>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const NArgs a) {
-  const int lane = threadIdx.x % 64, c = lane % LPR, g = lane / LPR;
-  constexpr int HPW = 64 / LPR;
-  long long unit = (long long)blockIdx.x * 4 + threadIdx.x / 64;
-  int k = 0;
-  const long long n0 = (long long)a.p[0].B * a.p[0].T * ((a.p[0].H + a.heads - 1) / a.heads);
-  if (unit >= n0) {
-    unit -= n0;
-    k = 1;
-  }
-  const NPart& q = a.p[k];
-  const int hu = (q.H + a.heads - 1) / a.heads;
-  if (unit >= (long long)q.B * q.T * hu) return;
-  const long long tok = unit / hu;
-  const int b = (int)(tok / q.T), t = (int)(tok % q.T);
-  const int h0 = (int)(unit % hu) * a.heads, h1 = min(q.H, h0 + a.heads);
-  const int p0 = c * V;
+  __shared__ float2 sc[4][64 * V];
+  using U = Unit<V, LPR>;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, p0 = lane % LPR * V;
+  int blk;
+  const NPart& q = a.p[n_part(a, blk)];
   const bool in = p0 < a.D / 2;
   using EI = typename Num<KI>::E;
   using EO = typename Num<KO>::E;
-
-  unsigned long long turn[V];
-  float w[2 * V], cs[V], sn[V];
+  const float inv = 1.f / (float)a.D;
+  float w[2 * V] = {};
+  if (in) n_load<1, V, CH>(a, q.w, p0, w);
+  const long long units = U::count(a, q);
+  for (long long unit = (long long)blk * 4 + wave; unit < units; unit += 4LL * q.blocks) {
+    const U n(a, q, unit, sc[wave]);
+    float sn[V], cs[V];
+    n.sines(q, sc[wave], sn, cs);
+    const EI* x = (const EI*)q.x + n.b * q.xb + n.t * q.xt;
+    EO* y = (EO*)q.y + n.b * q.yb + n.t * q.yt;
+    const bool live = in && n.valid;
+    // all lanes of a wave run the same number of rounds
+    for (int h = n.h0, base = 0; base < n.h1; h += n.step, base += n.step) {
+      float u[2 * V] = {};
+      const bool on = live && h < n.h1;
+      if (on) n_load<KI, V, CH>(a, x + h * q.xh, p0, u);
+      float ss = 0.f;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    turn[i] = p0 + i < a.R / 2 ? a.turn[p0 + i] : 0;
-    const bool e = p0 + i < a.D / 2;
-    w[i] = e ? q.w[n_first(a, p0 + i)] : 0.f;
-    w[V + i] = e ? q.w[n_second(a, p0 + i)] : 0.f;
-  }
-  n_angles<V>(a, q, b, t, p0, turn, cs, sn);
-  const EI* x = (const EI*)q.x + b * q.xb + t * q.xt;
-  EO* y = (EO*)q.y + b * q.yb + t * q.yt;
-  for (int h = h0 + g; h < h1; h += HPW) {
-    float u[2 * V] = {};
-    if (in) n_load<KI, V, CH>(a, x + h * q.xh, p0, u);
-    float ss = 0.f;
+      for (int i = 0; i < 2 * V; ++i) ss = fmaf(u[i], u[i], ss);
+      const float r = __frsqrt_rn(fmaf(n_sum<LPR>(ss), inv, a.eps));
+      float o[2 * V];
 #pragma unroll
-    for (int i = 0; i < 2 * V; ++i) ss = fmaf(u[i], u[i], ss);
-    const float r = __frsqrt_rn(n_sum<LPR>(ss) / (float)a.D + a.eps);
-    float o[2 * V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float ua = u[i] * r * w[i], ub = u[V + i] * r * w[V + i];
-      o[i] = ua * cs[i] - ub * sn[i];
-      o[V + i] = ub * cs[i] + ua * sn[i];
+      for (int i = 0; i < V; ++i) {
+        const float ua = u[i] * r * w[i], ub = u[V + i] * r * w[V + i];
+        o[i] = ua * cs[i] - ub * sn[i];
+        o[V + i] = ub * cs[i] + ua * sn[i];
+      }
+      if (on) n_store<KO, V, CH>(a, y + h * q.yh, p0, o);
     }
-    if (in) n_store<KO, V, CH>(a, y + h * q.yh, p0, o);
   }
 }
 
 // dx, and each block's share of dw.
 template <int KI, int KO, int V, int LPR, bool CH>
 __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(const NArgs a) {
-  constexpr int HPW = 64 / LPR;
-  __shared__ float red[4][2 * 64 * V];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = lane % LPR, g = lane / LPR;
-  const int k = (int)blockIdx.x >= a.p[0].blocks;
-  const NPart& q = a.p[k];
-  const int blk = k ? blockIdx.x - a.p[0].blocks : blockIdx.x;
-  const int hu = (q.H + a.heads - 1) / a.heads;
-  const long long units = (long long)q.B * q.T * hu;
-  const int p0 = c * V;
+  __shared__ float2 sc[4][64 * V];
+  using U = Unit<V, LPR>;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = lane % LPR, p0 = c * V;
+  int blk;
+  const NPart& q = a.p[n_part(a, blk)];
   const bool in = p0 < a.D / 2;
   using EI = typename Num<KI>::E;
   using EO = typename Num<KO>::E;
-
-  unsigned long long turn[V];
-  float w[2 * V], cs[V], sn[V], dw[2 * V] = {};
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    turn[i] = p0 + i < a.R / 2 ? a.turn[p0 + i] : 0;
-    const bool e = p0 + i < a.D / 2;
-    w[i] = e ? q.w[n_first(a, p0 + i)] : 0.f;
-    w[V + i] = e ? q.w[n_second(a, p0 + i)] : 0.f;
-  }
+  const float inv = 1.f / (float)a.D;
+  float w[2 * V] = {}, dw[2 * V] = {};
+  if (in) n_load<1, V, CH>(a, q.w, p0, w);
+  const long long units = U::count(a, q);
   for (long long unit = (long long)blk * 4 + wave; unit < units; unit += 4LL * q.blocks) {
-    const long long tok = unit / hu;
-    const int b = (int)(tok / q.T), t = (int)(tok % q.T);
-    const int h0 = (int)(unit % hu) * a.heads, h1 = min(q.H, h0 + a.heads);
-    n_angles<V>(a, q, b, t, p0, turn, cs, sn);
-    const EI* x = (const EI*)q.x + b * q.xb + t * q.xt;
-    const EO* dy = (const EO*)q.dy + b * q.gb + t * q.gt;
-    EI* dx = (EI*)q.y + b * q.yb + t * q.yt;
-    for (int h = h0 + g; h < h1; h += HPW) {
+    const U n(a, q, unit, sc[wave]);
+    float sn[V], cs[V];
+    n.sines(q, sc[wave], sn, cs);
+    const EI* x = (const EI*)q.x + n.b * q.xb + n.t * q.xt;
+    const EO* dy = (const EO*)q.dy + n.b * q.gb + n.t * q.gt;
+    EI* dx = (EI*)q.y + n.b * q.yb + n.t * q.yt;
+    const bool live = in && n.valid;
+    for (int h = n.h0, base = 0; base < n.h1; h += n.step, base += n.step) {
       float u[2 * V] = {}, d[2 * V] = {};
-      if (in) {
+      const bool on = live && h < n.h1;
+      if (on) {
         n_load<KI, V, CH>(a, x + h * q.xh, p0, u);
         n_load<KO, V, CH>(a, dy + h * q.gh, p0, d);
       }
       float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < 2 * V; ++i) ss = fmaf(u[i], u[i], ss);
-      const float r = __frsqrt_rn(n_sum<LPR>(ss) / (float)a.D + a.eps);
+      const float r = __frsqrt_rn(fmaf(n_sum<LPR>(ss), inv, a.eps));
       float dot = 0.f;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float da = d[i] * cs[i] + d[V + i] * sn[i], db = d[V + i] * cs[i] - d[i] * sn[i];
-        u[i] *= r;
-        u[V + i] *= r;
+        u[i] = on ? u[i] * r : 0.f;          // eps = 0: no row, no infinity
+        u[V + i] = on ? u[V + i] * r : 0.f;
         dw[i] = fmaf(da, u[i], dw[i]);
         dw[V + i] = fmaf(db, u[V + i], dw[V + i]);
         d[i] = da * w[i];
         d[V + i] = db * w[V + i];
         dot = fmaf(d[i], u[i], fmaf(d[V + i], u[V + i], dot));
       }
-      dot = n_sum<LPR>(dot) / (float)a.D;
+      dot = n_sum<LPR>(dot) * inv;
 #pragma unroll
       for (int i = 0; i < 2 * V; ++i) d[i] = r * (d[i] - u[i] * dot);
-      if (in) n_store<KI, V, CH>(a, dx + h * q.yh, p0, d);
+      if (on) n_store<KI, V, CH>(a, dx + h * q.yh, p0, d);
     }
   }
   if (!a.part) return;
+  __syncthreads();
+  float* red = (float*)sc;                            // [4][2 V LPR]
 #pragma unroll
   for (int i = 0; i < 2 * V; ++i) {
 #pragma unroll
     for (int m = LPR; m < 64; m <<= 1) dw[i] += __shfl_xor(dw[i], m);
-    if (g == 0) red[wave][i * LPR + c] = dw[i];
+    if (lane < LPR) red[wave * (2 * V * LPR) + i * LPR + c] = dw[i];
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * V * LPR; i += 256) {
     const int p = i % LPR * V + i / LPR % V;
     if (p < a.D / 2)
       a.part[(long long)blockIdx.x * a.D + (i / LPR < V ? n_first(a, p) : n_second(a, p))] =
-          red[0][i] + red[1][i] + red[2][i] + red[3][i];
+          red[i] + red[2 * V * LPR + i] + red[4 * V * LPR + i] + red[6 * V * LPR + i];
   }
 }
 
@@ -353,20 +380,23 @@ bool n_chunked(int type, int D, int R, int interleaved) {
   const int v = n_vec(type);
   return interleaved ? D / 2 % v == 0 : R / 2 % v == 0 && (D - R) / 2 % v == 0;
 }
+// lanes per head
 int n_lanes(int type, int D, bool ch) {
-  const int v = ch ? n_vec(type) : 2, n = (D / 2 + v - 1) / v;
-  return n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 ? 32 : 64;
+  if (!ch) return D <= 64 ? 16 : 64;                // two pairs each
+  const int v = n_vec(type), n = (D / 2 + v - 1) / v;
+  return n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : 32;
 }
 
 template <int KI, int KO>
 int n_run(const NArgs& a, int grid, bool bwd, bool ch, int lpr, hipStream_t st) {
   constexpr int V = n_vec(KI);
   if (ch) {
+    if (lpr == 4) return n_go<KI, KO, V, 4, true>(a, grid, bwd, st);
     if (lpr == 8) return n_go<KI, KO, V, 8, true>(a, grid, bwd, st);
     if (lpr == 16) return n_go<KI, KO, V, 16, true>(a, grid, bwd, st);
     return n_go<KI, KO, V, 32, true>(a, grid, bwd, st);
   }
-  if (lpr <= 16) return n_go<KI, KO, 2, 16, false>(a, grid, bwd, st);
+  if (lpr == 16) return n_go<KI, KO, 2, 16, false>(a, grid, bwd, st);
   return n_go<KI, KO, 2, 64, false>(a, grid, bwd, st);
 }
 
@@ -380,29 +410,29 @@ int n_dispatch(const NArgs& a, int grid, bool bwd, bool ch, int lpr, int ti, int
   return 1002;
 }
 
-// heads per unit: a whole token per wave shares its sines among the heads;
-// with few tokens the heads go to waves of their own
-int n_heads(long long tokens, int H, int lpr) {
-  const int at_once = 64 / lpr;
-  return tokens >= 8192 ? (H + at_once - 1) / at_once * at_once : at_once;
+// Units of a part (Unit::count)
+long long n_units(const NArgs& a, const NPart& p, int lpr) {
+  const long long tokens = (long long)p.B * p.T, at_once = 64 / lpr >> p.lg;
+  return (tokens + at_once - 1) / at_once * (a.many ? 1 : (p.H + (1 << p.lg) - 1) >> p.lg);
 }
-long long n_units(const NPart& p, int heads) {
-  return (long long)p.B * p.T * ((p.H + heads - 1) / heads);
-}
-// blocks of the backward for both parts (at most 1024 in all, shared by size)
-void n_blocks(NArgs& a) {
-  const long long u0 = n_units(a.p[0], a.heads), u1 = n_units(a.p[1], a.heads);
-  const long long b0 = (u0 + 3) / 4, b1 = (u1 + 3) / 4, all = b0 + b1;
-  if (all <= 1024) {
+// Blocks for both parts, at most `most`, shared by the heads that they have:
+// a wave with several units loads its weights once.
+void n_blocks(NArgs& a, int lpr, int most) {
+  const long long u0 = n_units(a, a.p[0], lpr), u1 = n_units(a, a.p[1], lpr);
+  const long long b0 = (u0 + 3) / 4, b1 = (u1 + 3) / 4;
+  if (b0 + b1 <= most) {
     a.p[0].blocks = (int)b0;
     a.p[1].blocks = (int)b1;
-  } else {
-    long long x = 1024 * b0 / all;
-    if (x < 1 && b0) x = 1;
-    if (x > 1023 && b1) x = 1023;
-    a.p[0].blocks = (int)x;
-    a.p[1].blocks = (int)(1024 - x);
+    return;
   }
+  const double r0 = (double)a.p[0].B * a.p[0].T * a.p[0].H;
+  const double r1 = (double)a.p[1].B * a.p[1].T * a.p[1].H;
+  long long x = (long long)(most * (r0 / (r0 + r1)));
+  if (b1 && x > most - 1) x = most - 1;
+  if (b0 && x < 1) x = 1;
+  if (x > b0) x = b0;
+  a.p[0].blocks = (int)x;
+  a.p[1].blocks = (int)(most - x < b1 ? most - x : b1);
 }
 
 bool n_fill(NArgs& a, const long long* s, const void* q, const void* k, const void* gq,
@@ -417,9 +447,10 @@ bool n_fill(NArgs& a, const long long* s, const void* q, const void* k, const vo
     const long long* t = s + 15 * i;
     NPart& p = a.p[i];
     p = NPart{x[i], t[3], t[4], t[5], g[i], t[6], t[7], t[8], y[i], t[9],
-              t[10], t[11], w[i], pos[i], t[12], t[13], t[14], (int)t[0], (int)t[1], (int)t[2], 0};
+              t[10], t[11], w[i], pos[i], t[12], t[13], t[14], (int)t[0], (int)t[1], (int)t[2], 0, 0};
     for (int j = 0; j < 3; ++j)
       if (t[j] < 0 || t[j] > 0x7fffffffLL) return false;
+    if (t[0] * t[1] > 0x7fffffffLL) return false;
     if (!x[i]) p.B = p.T = p.H = 0;
     else if (!y[i] || !w[i]) return false;
   }
@@ -457,23 +488,19 @@ static int n_entry(const void* q, const void* k, const void* gq, const void* gk,
   a.pos32 = pos32;
   a.eps = eps;
   const bool ch = n_chunked(ti, D, R, interleaved);
-  int lpr = n_lanes(ti, D, ch);
-  if (!ch) lpr = lpr <= 16 ? 16 : 64;
-  const long long tokens =
-      (long long)a.p[0].B * a.p[0].T + (long long)a.p[1].B * a.p[1].T;
-  const int H = a.p[0].H > a.p[1].H ? a.p[0].H : a.p[1].H;
-  a.heads = n_heads(tokens, H < 1 ? 1 : H, lpr);
-  const long long units = n_units(a.p[0], a.heads) + n_units(a.p[1], a.heads);
-  if (units > 0x1ffffffffLL) return 1001;
-  const hipStream_t st = (hipStream_t)stream;
-  if (!bwd) {
-    if (!units) return 0;
-    return n_dispatch(a, (int)((units + 3) / 4), false, ch, lpr, ti, to, st);
+  const int lpr = n_lanes(ti, D, ch);
+  long long tokens = 0;
+  for (NPart& p : a.p) {
+    while ((1 << p.lg) < p.H && (1 << p.lg) < 64 / lpr) ++p.lg;
+    tokens += (long long)p.B * p.T;
   }
-  n_blocks(a);
+  // with few tokens the heads of one go to waves of their own
+  a.many = tokens >= 8192;
+  const hipStream_t st = (hipStream_t)stream;
+  n_blocks(a, lpr, bwd ? 1024 : 4096);
   const int grid = a.p[0].blocks + a.p[1].blocks;
   if (grid)
-    if (const int e = n_dispatch(a, grid, true, ch, lpr, ti, to, st)) return e;
+    if (const int e = n_dispatch(a, grid, bwd, ch, lpr, ti, to, st)) return e;
   if (!part) return 0;
   hipLaunchKernelGGL(qk_norm_rope_dw_kernel, dim3((D + 7) / 8, 2), dim3(256), 0, st, part,
                      a.p[0].blocks, a.p[1].blocks, D, dwq, dwk);

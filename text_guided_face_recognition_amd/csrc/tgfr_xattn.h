@@ -345,19 +345,63 @@ struct MemSrc {
 struct XWork {
   int b, g, bh, tile, split;
 };
-__device__ __forceinline__ XWork x_work(const XArgs& a) {
-  // Consecutive work shares K and V (or Q and dO), and so one XCD's L2.  With
-  // lengths, whole samples per XCD would leave the XCDs of short ones idle:
-  // they get runs of four.
-  const int total = gridDim.x, L = blockIdx.x, q = L / 8;
-  const int id = !(a.q_lens || a.kv_lens) ? xcd_remap(L, total)
-                 : L < total / 32 * 32    ? (q / 4 * 8 + L % 8) * 4 + q % 4
-                                          : L;
+// Place L of `total` along the blocks: consecutive places share K and V (or Q
+// and dO), and so should share one XCD's L2.  Where streams differ in length,
+// whole samples per XCD would leave the XCDs of short ones idle: runs of four.
+__device__ __forceinline__ int x_place(int L, int total, bool ragged) {
+  if (!ragged) return xcd_remap(L, total);
+  const int q = L / 8;
+  return L < total / 32 * 32 ? (q / 4 * 8 + L % 8) * 4 + q % 4 : L;
+}
+// own, stream: lengths (or NULL) of what the waves own, of `per` items per tile
+// (tokens of Q count G rows), and of what they stream.
+__device__ __forceinline__ XWork x_work(const XArgs& a, const int* own, int T, int G, int per,
+                                        const int* stream) {
   XWork w;
-  w.tile = id % a.tiles;
-  const int rest = id / a.tiles;
-  w.bh = rest % (a.B * a.Hk);
-  w.split = rest / (a.B * a.Hk);
+  const int L = blockIdx.x, heads = a.Hk * a.splits;
+  if (!own) {
+    const int id = x_place(L, gridDim.x, stream);
+    w.tile = id % a.tiles;
+    const int rest = id / a.tiles;
+    w.bh = rest % (a.B * a.Hk);
+    w.split = rest / (a.B * a.Hk);
+  } else {
+    // Tiles of padding only clear their results: they come last, so that the
+    // others spread evenly over the CUs.  Lane i counts sample b0 + i's tiles.
+    const int lane = threadIdx.x % 64;
+    auto tiles_of = [&](int b) {
+      return b < a.B ? (min(max(own[b], 0), T) * G + per - 1) / per : 0;
+    };
+    int live = 0;
+    for (int b = lane; b < a.B; b += 64) live += tiles_of(b);
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) live += __shfl_xor(live, m);
+    live *= heads;
+    const bool pad = L >= live;
+    const int id = pad ? L - live : x_place(L, live, stream);
+    int before = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      const int b = b0 + lane, used = tiles_of(b);
+      const int n = b < a.B ? (pad ? a.tiles - used : used) : 0;
+      int sum = n;                                       // of the samples up to b
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) {
+        const int up = __shfl_up(sum, m);
+        if (lane >= m) sum += up;
+      }
+      const int lo = (before + sum - n) * heads;
+      const uint64_t at = __ballot(id >= lo && id < lo + n * heads);
+      if (at) {
+        const int k = __builtin_ctzll(at);
+        const int r = id - __shfl(lo, k), nk = __shfl(n, k), rest = r / nk;
+        w.tile = r % nk + (pad ? __shfl(used, k) : 0);
+        w.bh = (b0 + k) * a.Hk + rest % a.Hk;
+        w.split = rest / a.Hk;
+        break;
+      }
+      before += __shfl(sum, 63);
+    }
+  }
   w.b = w.bh / a.Hk;
   w.g = w.bh % a.Hk;
   // (division runs on the vector unit; these are the same in all lanes)
@@ -765,7 +809,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(
   using S = KeyStream<T, DP, WR, WS, DS, true>;
   using I = Img<T, S::DH>;
   using E = typename T::elem;
-  const XWork w = x_work(a);
+  const XWork w = x_work(a, a.q_lens, a.Tq, a.G, 32 * WR, a.kv_lens);
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const int wr = wave % WR, ws = wave / WR % WS, ds = wave / (WR * WS);
   const int lr = lane & 31, h = lane >> 5;
@@ -879,32 +923,43 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(
   }
 }
 
-// Joins the splits of the forward: one wave per row.
-template <class T>
+// Joins the splits of the forward: a block per row, 256 / W threads sharing
+// each of the W >= D columns.
+template <class T, int W>
 __global__ __launch_bounds__(256) void xattn_fwd_join(const XArgs a) {
   using E = typename T::elem;
-  const int lane = threadIdx.x % 64;
-  const long long n = (long long)a.B * a.Hk * a.R;
-  const long long id = (long long)blockIdx.x * 4 + threadIdx.x / 64;
-  if (id >= n) return;
-  const int bh = (int)(id / a.R), r = (int)(id % a.R);
-  float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * n + id)]);
+  constexpr int P = 256 / W;
+  __shared__ float part[256], top[P];
+  const long long n = (long long)a.B * a.Hk * a.R, id = blockIdx.x;
+  const int bh = (int)(id / a.R), r = (int)(id % a.R), lane = threadIdx.x % 64;
+  const int d = threadIdx.x % W, p = threadIdx.x / W;
+  float m = -INFINITY, l = 0.f, o = 0.f;
+  for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, a.part_ml[2 * (s * n + id)]);
+  m = wave_max(m);
   const float mu = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o[4] = {};
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (s * n + id)] - mu);
-    l += f * a.part_ml[2 * (s * n + id) + 1];
+#pragma unroll 4
+  for (int s = p; s < a.splits; s += P) {
+    const float2 ml = *(const float2*)(a.part_ml + 2 * (s * n + id));
+    const float f = __builtin_amdgcn_exp2f(ml.x - mu);
+    l = fmaf(f, ml.y, l);
+    if (d < a.D) o = fmaf(f, a.part[(s * n + id) * a.D + d], o);
+  }
+  if constexpr (P > 1) {
+    part[threadIdx.x] = o;
+    if (d == 0) top[p] = l;
+    __syncthreads();
+    if (p) return;
+    o = l = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (lane + 64 * k < a.D) o[k] += f * a.part[(s * n + id) * a.D + lane + 64 * k];
+    for (int i = 0; i < P; ++i) {
+      o += part[i * W + d];
+      l += top[i];
+    }
   }
   const bool none = m == -INFINITY && l == 0.f;
-  if (a.lse && lane == 0) a.lse[id] = none ? INFINITY : m + __builtin_amdgcn_logf(l);
-  E* p = x_row<E>(a.o, bh / a.Hk, bh % a.Hk, a.G, r);
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (lane + 64 * k < a.D) p[lane + 64 * k] = T::bits(none ? 0.f : o[k] / l);
+  if (a.lse && d == 0) a.lse[id] = none ? INFINITY : m + __builtin_amdgcn_logf(l);
+  if (d < a.D)
+    x_row<E>(a.o, bh / a.Hk, bh % a.Hk, a.G, r)[d] = T::bits(none ? 0.f : o / l);
 }
 
 // ----------------------------------------------------------------- backward ---
@@ -927,7 +982,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(c
   using S = KeyStream<T, DP, WR, WS, DS, false>;
   using I = Img<T, S::DH>;
   using E = typename T::elem;
-  const XWork w = x_work(a);
+  const XWork w = x_work(a, a.q_lens, a.Tq, a.G, 32 * WR, a.kv_lens);
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const int wr = wave % WR, ws = wave / WR % WS, ds = wave / (WR * WS);
   const int lr = lane & 31, h = lane >> 5;
@@ -1057,9 +1112,9 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(c
 
 // dK and dV of WC * 32 states, streaming Q and dO, 32 WS rows at a time; WS
 // waves share the states and take different rows, DS waves the columns of the
-// results: of fp32 as above, of 16-bit types with 256 columns because both
-// accumulators are too large for one wave's registers (each of the two forms
-// all of the scores, 6 products where 4 would do).
+// results: of fp32 as above, of 16-bit types because both accumulators are too
+// large for one wave's registers (each of the two forms all of the scores, 6
+// products where 4 would do).
 template <class T, int DP, int WC, int WS, int DS>
 struct DkvCfg {
   static constexpr int NT = 64 * WC * WS * DS, RT = 32 * WS, AHEAD = T::ES == 4 ? 8 : 4;
@@ -1080,7 +1135,7 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
   constexpr int DH = DP / DS, NB = DH / 32, DO = C::MEM ? DH : DP;
   using I = Img<T, DO>;
   using E = typename T::elem;
-  const XWork w = x_work(a);
+  const XWork w = x_work(a, a.kv_lens, a.Tk, 1, 32 * WC, a.q_lens);
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const int wc = wave % WC, ws = wave / WC % WS, ds = wave / (WC * WS);
   const int lr = lane & 31, h = lane >> 5;
@@ -1329,23 +1384,33 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
   }
 }
 
-// Sums the splits of a gradient, one wave per row: dQ (n rows = R), or dK and
-// dV (blockIdx.y, n rows = Tk).
-template <class T, bool KV>
+// Sums the splits of a gradient, as the forward's are joined: dQ (R rows), or
+// dK and dV (blockIdx.y; Tk rows).
+template <class T, int W, bool KV>
 __global__ __launch_bounds__(256) void xattn_join(const XArgs a) {
   using E = typename T::elem;
-  const int lane = threadIdx.x % 64, per = KV ? a.Tk : a.R;
-  const long long n = (long long)a.B * a.Hk * per;
-  const long long id = (long long)blockIdx.x * 4 + threadIdx.x / 64;
-  if (id >= n) return;
+  constexpr int P = 256 / W;
+  __shared__ float sum[256];
+  const int per = KV ? a.Tk : a.R;
+  const long long n = (long long)a.B * a.Hk * per, id = blockIdx.x;
   const int bh = (int)(id / per), r = (int)(id % per), b = bh / a.Hk, g = bh % a.Hk;
+  const int d = threadIdx.x % W, p = threadIdx.x / W;
   const float* part = a.part + (KV ? blockIdx.y * a.splits * n * a.D : 0);
-  E* p = KV ? x_key<E>(blockIdx.y ? a.dv : a.dk, b, g, r) : x_row<E>(a.dq, b, g, a.G, r);
-  for (int d = lane; d < a.D; d += 64) {
-    float x = 0.f;
-    for (int s = 0; s < a.splits; ++s) x += part[(s * n + id) * a.D + d];
-    p[d] = T::bits(x);
+  float x = 0.f;
+  if (d < a.D) {
+#pragma unroll 4
+    for (int s = p; s < a.splits; s += P) x += part[(s * n + id) * a.D + d];
   }
+  if constexpr (P > 1) {
+    sum[threadIdx.x] = x;
+    __syncthreads();
+    if (p) return;
+    x = 0.f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) x += sum[i * W + d];
+  }
+  E* to = KV ? x_key<E>(blockIdx.y ? a.dv : a.dk, b, g, r) : x_row<E>(a.dq, b, g, a.G, r);
+  if (d < a.D) to[d] = T::bits(x);
 }
 
 // ------------------------------------------------------------------- launch ---
@@ -1354,21 +1419,26 @@ enum { X_FWD, X_DQ, X_DKV };
 struct XPlan {
   int waves, tiles, splits;      // waves that own rows (dK, dV: states), 32 each
 };
-// Waves along the columns: fp32 64 columns each; dK, dV of 16-bit types with
-// 256 columns two waves.
+// Waves along the columns: fp32 64 columns each; dK, dV of 16-bit types two
+// waves from 128 columns on (at 128, two waves per SIMD of 24 products a piece
+// each took 0.6 of the time of one wave of 32, whose registers leave no room
+// for a second).
 constexpr int x_columns(int type, int what, int dp) {
-  return type == 1 ? dp / 64 : what == X_DKV && dp == 256 ? 2 : 1;
+  return type == 1 ? dp / 64 : what == X_DKV && dp >= 128 ? 2 : 1;
 }
 // Least waves that own rows (states): the rings of fewer would pass the LDS.
 constexpr int x_least(int type, int what, int dp) {
-  return type == 1 || dp <= 64 ? 1 : dp == 128 || what == X_DKV ? 2 : 4;
+  return type == 1 || dp <= 64 ? 1 : what == X_DKV ? dp / 128 : dp == 128 ? 2 : 4;
 }
 // The split of one kernel's work.  `own` rows (dK, dV: states) belong to the
 // waves, the others are streamed.  A block's four waves (or those that the
-// columns leave) own 32 rows each while that leaves two blocks per CU; below,
+// columns leave) own 32 rows each while that gives every CU a block; below,
 // two or all of them share rows and take different parts of the stream, where
-// that has a piece of 32 for each, and below that the stream is split over
-// blocks, whose results a second launch joins.
+// that has a piece of 32 for each (1 x 2048 x 2048 of 8 heads on one: 38 us
+// against 48; 8 x 64 x 512, 8 heads of 64: 10.0 against 12.8).  What still
+// leaves CUs without a block splits the stream over blocks, 256 items or more
+// each, whose results a second launch joins (17 tokens of 8 heads on 8192
+// states: 32 us against 114; not at 99 blocks: 22 both ways).
 inline XPlan x_plan(const XArgs& a, int type, int what) {
   const int own = what == X_DKV ? a.Tk : a.R, stream = what == X_DKV ? a.R : a.Tk;
   const long long heads = (long long)a.B * a.Hk;
@@ -1376,13 +1446,13 @@ inline XPlan x_plan(const XArgs& a, int type, int what) {
   XPlan p;
   for (p.waves = all;; p.waves /= 2) {
     p.tiles = (own + 32 * p.waves - 1) / (32 * p.waves);
-    if (p.waves == x_least(type, what, dp) || (p.tiles * heads >= 512 && own > 16 * p.waves) ||
+    if (p.waves == x_least(type, what, dp) || p.tiles * heads >= 256 ||
         stream <= 32 * (all / p.waves))
       break;
   }
   const long long blocks = p.tiles * heads;
-  const int step = type == 1 ? 32 * (all / p.waves) : 128, most = (stream + step - 1) / step;
-  const long long want = blocks >= 384 ? 1 : (512 + blocks - 1) / blocks;
+  const int each = type == 1 ? 64 : 256, most = (stream + each - 1) / each;
+  const long long want = blocks >= (own <= 32 ? 256 : 96) ? 1 : (255 + blocks) / blocks;
   p.splits = (int)(want < most ? want : most);
   return p;
 }
@@ -1411,7 +1481,8 @@ template <class T, int DP, int W>
 int x_states(const XArgs& a, void* stream) {
   constexpr int DS = x_columns(T::TYPE, X_DKV, DP), WS = 4 / DS / W;
   using C = DkvCfg<T, DP, W, WS, DS>;
-  return x_go(xattn_dkv<T, DP, W, WS, DS, 1>, a, a.splits > 1 ? C::LDS32 : C::LDS, C::NT, stream);
+  constexpr int OCC = T::ES == 2 && DP <= 128 && C::FED <= 80 * 1024 ? 2 : 1;
+  return x_go(xattn_dkv<T, DP, W, WS, DS, OCC>, a, a.splits > 1 ? C::LDS32 : C::LDS, C::NT, stream);
 }
 template <class T, int DP, int W>
 int x_waves(const XArgs& a, int waves, int what, void* stream) {
@@ -1434,16 +1505,15 @@ int x_run(XArgs a, int what, void* stream) {
   const XPlan p = x_plan(a, T::TYPE, what);
   a.tiles = p.tiles;
   a.splits = p.splits;
-  const int nrow = a.B * a.Hk * (what == X_DKV ? a.Tk : a.R);
   const int e = x_waves<T, DP, 4>(a, p.waves, what, stream);
   if (e || a.splits == 1) return e;
-  const dim3 grid((nrow + 3) / 4, what == X_DKV ? 2 : 1);
+  const dim3 grid((unsigned)(a.B * a.Hk * (what == X_DKV ? a.Tk : a.R)), what == X_DKV ? 2 : 1);
   if (what == X_FWD)
-    hipLaunchKernelGGL((xattn_fwd_join<T>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL((xattn_fwd_join<T, DP>), grid, dim3(256), 0, (hipStream_t)stream, a);
   else if (what == X_DQ)
-    hipLaunchKernelGGL((xattn_join<T, false>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL((xattn_join<T, DP, false>), grid, dim3(256), 0, (hipStream_t)stream, a);
   else
-    hipLaunchKernelGGL((xattn_join<T, true>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL((xattn_join<T, DP, true>), grid, dim3(256), 0, (hipStream_t)stream, a);
   return (int)hipGetLastError();
 }
 

@@ -96,8 +96,8 @@ int tgfr_cross_attention_fwd(const void* q, const void* k, const void* v, void* 
   a.scale = scale;
   a.lse = lse;
   if (n) {
-    a.part = ws;
-    a.part_ml = ws + n / (D + 2) * D;
+    a.part_ml = ws;
+    a.part = ws + 2 * (n / (D + 2));
   }
   return x_dispatch(a, type, X_FWD, stream);
 }
