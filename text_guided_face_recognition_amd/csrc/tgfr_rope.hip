@@ -192,6 +192,7 @@ struct Unit {
     h1 = a.many ? q.H : min(q.H, (hc + 1) * step);
     valid = first + (g >> q.lg) < tokens;
     token(q, min(first + (g >> q.lg), tokens - 1), b, t);
+    asm volatile("" ::: "memory");                    // the last unit's are read
     // Sines: 64 / (tokens of the wave) lanes per token, pair after pair.
     const int per = LPR << q.lg;                      // lanes per token
     int sb, st;
@@ -212,7 +213,7 @@ struct Unit {
       }
       sc[lane / per * (LPR * V) + p] = v;
     }
-    __builtin_amdgcn_wave_barrier();                  // (one wave's LDS is in order)
+    asm volatile("" ::: "memory");                    // (one wave's LDS is in order)
   }
   __device__ __forceinline__ void sines(const NPart& q, const float2* sc, float (&sn)[V],
                                         float (&cs)[V]) const {

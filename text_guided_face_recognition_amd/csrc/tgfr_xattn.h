@@ -199,9 +199,13 @@ __device__ __forceinline__ uint32_t buf4(__amdgpu_buffer_rsrc_t r, uint32_t off)
   return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
 }
 
-// 16 (4) bytes per lane from a scalar base + lane offset straight to LDS byte
-// `to` (wave-uniform) + 16 (4) * lane.  Inline asm, so that the compiler sees no
+// 16 bytes per lane from a scalar base + lane offset (4 from an address) straight
+// to LDS byte `to` (wave-uniform) + 16 (4) * lane.  Inline asm, so that the compiler sees no
 // LDS write pending on the memory counter; the kernels wait by count (glds16).
+// zeros for places that are not read, then the statistics of such rows (log
+// sum +infinity: probability 0; delta 0)
+static __device__ const float x_pad[8] __attribute__((aligned(16))) = {
+    0.f, 0.f, 0.f, 0.f, INFINITY, 0.f, 0.f, 0.f};
 __device__ __forceinline__ const void* scalar(const void* p) {
   const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)p);
   const uint64_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)((uintptr_t)p >> 32));
@@ -213,10 +217,9 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t t
                "s"(scalar(base)), "s"(m0)
                : "memory", "m0");
 }
-__device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t to) {
+__device__ __forceinline__ void dma4(const float* src, uint32_t to) {
   const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_base() + to));
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off),
-               "s"(scalar(base)), "s"(m0)
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(m0)
                : "memory", "m0");
 }
 
@@ -254,20 +257,27 @@ struct Feed {
     for (int n = 0; n < N; ++n)
       if (off[n] == NONE) lds_st16(base + place(n), zero16());
   }
-  // starts a whole tile (FULL), or one of `rows` rows, whose first is at p: N
-  // DMA instructions per wave for a whole tile
-  template <bool FULL>
-  __device__ __forceinline__ void start(const void* p, int rows, uint32_t base) const {
+  // starts a whole tile whose first row is at p; N DMA instructions per wave
+  __device__ __forceinline__ void start(const void* p, uint32_t base) const {
     const uint32_t to = base + 16 * (threadIdx.x & ~63u);
     if (whole) {
 #pragma unroll
-      for (int n = 0; n < N; ++n)
-        if (FULL || row(n) < rows) dma16(p, off[n], to + 16 * NT * n);
+      for (int n = 0; n < N; ++n) dma16(p, off[n], to + 16 * NT * n);
     } else {       // an instruction covers whole rows: some lanes always take part
 #pragma unroll
       for (int n = 0; n < N; ++n)
-        if (off[n] != NONE && (FULL || row(n) < rows)) dma16(p, off[n], to + 16 * NT * n);
+        if (off[n] != NONE) dma16(p, off[n], to + 16 * NT * n);
     }
+  }
+  // the same with zeros for the rows that are not kept(row), which are not
+  // read: their lanes fetch zeros from x_pad
+  template <class Kept>
+  __device__ __forceinline__ void start_kept(const void* p, Kept kept, uint32_t base) const {
+    const uint32_t to = base + 16 * (threadIdx.x & ~63u);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      glds16(off[n] != NONE && kept(row(n)) ? (const char*)p + off[n] : (const char*)x_pad,
+             to + 16 * NT * n);
   }
   // the same for rows at any alignment and of any length, through registers:
   // at(i) points to row i of the tile, or is NULL for zeros
@@ -278,13 +288,6 @@ struct Feed {
       const typename T::elem* p = at(row(n));
       lds_st16(base + place(n), p && chunk(n) * I::E < D ? ld_chunk<T>(p, chunk(n), D) : zero16());
     }
-  }
-  // zeros in the rows that gone(row) names
-  template <class Gone>
-  __device__ __forceinline__ void drop(Gone gone, uint32_t base) const {
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-      if (gone(row(n))) lds_st16(base + place(n), zero16());
   }
 };
 
@@ -611,7 +614,8 @@ struct KeyStream {
   using E = typename T::elem;
   static constexpr int NT = 64 * WR * WS * DS, KT = 32 * WS, DH = DP / DS;
   static constexpr bool MEM = T::ES == 4;
-  static constexpr int N = FWD ? 1 : 2, AHEAD = MEM ? 8 : 4;
+  // operands read ahead: as many as the registers hold
+  static constexpr int N = FWD ? 1 : 2, AHEAD = MEM ? 8 : FWD || DP == 64 ? 4 : 2;
   static constexpr int TILE = MEM ? 0 : I::bytes(KT), SLOT = 2 * TILE;
   // the ring and the mask's bits (fp32: two exchanges of 8 KiB per wave);
   // later the result
@@ -673,14 +677,6 @@ struct KeyStream {
       fv.clear(i * SLOT + TILE);
     }
     const int np = (khi - klo + KT - 1) / KT, full = (khi - klo) / KT;
-    if (mask) {
-      for (int j = klo + (threadIdx.x & ~63); j < khi; j += NT) {
-        const uint64_t b = __ballot(j + lane < khi && mask[j + lane]);
-        if (lane < 2)
-          *(LDS_AS uint32_t*)(lds_base() + BITS + 4 * ((j - klo) / 32 + lane)) = b >> (32 * lane);
-      }
-      __syncthreads();
-    }
     // kept bits of 32 states from klo + 32 i on (any i), the same in all lanes
     auto bits = [&](int i) X_INLINE -> uint32_t {
       const int left = khi - klo - 32 * i;
@@ -694,15 +690,36 @@ struct KeyStream {
       const int k0 = klo + n * KT;
       const uint32_t l0 = (n & 3) * SLOT;
       if (n >= np) return;
-      if (!a.fast_k) {
-        fk.copy([&](int r) { return k0 + r < khi ? K + (k0 + r) * a.k.st : nullptr; }, a.D, l0);
-        fv.copy([&](int r) { return k0 + r < khi ? V + (k0 + r) * a.v.st : nullptr; }, a.D,
-                l0 + TILE);
+      if (a.fast_k && !mask && n < full) {
+        fk.start(K + k0 * a.k.st, l0);
+        fv.start(V + k0 * a.v.st, l0 + TILE);
+        return;
+      }
+      uint32_t kb[WS];
+#pragma unroll
+      for (int i = 0; i < WS; ++i) kb[i] = bits(n * WS + i);
+      auto kept = [&](int r) X_INLINE {
+        uint32_t word = kb[0];
+#pragma unroll
+        for (int i = 1; i < WS; ++i) word = r >> 5 == i ? kb[i] : word;
+        return (word >> (r & 31)) & 1;
+      };
+      if (a.fast_k) {
+        fk.start_kept(K + k0 * a.k.st, kept, l0);
+        fv.start_kept(V + k0 * a.v.st, kept, l0 + TILE);
       } else {
-        fk.template start<false>(K + k0 * a.k.st, khi - k0, l0);
-        fv.template start<false>(V + k0 * a.v.st, khi - k0, l0 + TILE);
+        fk.copy([&](int r) X_INLINE { return kept(r) ? K + (k0 + r) * a.k.st : nullptr; }, a.D, l0);
+        fv.copy([&](int r) X_INLINE { return kept(r) ? V + (k0 + r) * a.v.st : nullptr; }, a.D, l0 + TILE);
       }
     };
+    if (mask) {
+      for (int j = klo + (threadIdx.x & ~63); j < khi; j += NT) {
+        const uint64_t b = __ballot(j + lane < khi && mask[j + lane]);
+        if (lane < 2)
+          *(LDS_AS uint32_t*)(lds_base() + BITS + 4 * ((j - klo) / 32 + lane)) = b >> (32 * lane);
+      }
+      __syncthreads();
+    }
     feed(0);
     feed(1);
     feed(2);
@@ -711,22 +728,13 @@ struct KeyStream {
         ring_barrier<2 * F::N>();            // all but piece n + 2
         const int k0 = klo + (n + 3) * KT;
         const uint32_t l0 = ((n + 3) & 3) * SLOT;
-        fk.template start<true>(K + k0 * a.k.st, KT, l0);
-        fv.template start<true>(V + k0 * a.v.st, KT, l0 + TILE);
+        fk.start(K + k0 * a.k.st, l0);
+        fv.start(V + k0 * a.v.st, l0 + TILE);
       } else {
-        if (a.fast_k && n >= 0 && n + 2 < full)
+        if (a.fast_k && n >= 0 && n + 2 < np)
           ring_barrier<2 * F::N>();
         else
           ring_barrier<0>();
-        bool all = true;
-#pragma unroll
-        for (int i = 0; i < WS; ++i) all = all && bits((n + 1) * WS + i) == 0xffffffffu;
-        if (!all && n + 1 < np) {
-          auto gone = [&](int r) { return !((bits((n + 1) * WS + (r >> 5)) >> (r & 31)) & 1); };
-          fk.drop(gone, ((n + 1) & 3) * SLOT);
-          fv.drop(gone, ((n + 1) & 3) * SLOT + TILE);
-          __syncthreads();
-        }
         if (n >= 0) feed(n + 3);
       }
     };
@@ -1281,11 +1289,13 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
     // same places), so that all waves count the same instructions
     auto stats = [&](int r0, uint32_t l0) X_INLINE {
 #pragma unroll
-      for (int i = 0; i < STATS; ++i)
-        if (64 * i + lane < RT && r0 + 64 * i + lane < rhi) {
-          dma4(a.lse + at + r0, 4 * (64 * i + lane), l0 + L0 + 256 * i);
-          dma4(a.delta + at + r0, 4 * (64 * i + lane), l0 + T0 + 256 * i);
+      for (int i = 0; i < STATS; ++i) {
+        const int r = r0 + 64 * i + lane;
+        if (64 * i + lane < RT) {
+          dma4(r < rhi ? a.lse + at + r : x_pad + 4, l0 + L0 + 256 * i);
+          dma4(r < rhi ? a.delta + at + r : x_pad, l0 + T0 + 256 * i);
         }
+      }
     };
     // a tile's first row, where G, a power of two, divides RT
     const int sh = 31 - __builtin_clz(a.G);
@@ -1297,14 +1307,21 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
       const uint32_t l0 = (n & 3) * C::TILE;
       if (n >= np) return;
       stats(r0, l0);
+      auto kept = [&](int r) X_INLINE { return r0 + r < rhi; };
       if (!a.fast_q) {
-        fq.copy([&](int r) {
-          return r0 + r < rhi ? x_row<E>(a.q, w.b, w.g, a.G, r0 + r) : nullptr; }, a.D, l0);
-        fd.copy([&](int r) {
-          return r0 + r < rhi ? x_row<E>(a.dout, w.b, w.g, a.G, r0 + r) : nullptr; }, a.D, l0 + D0);
+        auto row = [&](const XView& v) X_INLINE {
+          return [&](int r) X_INLINE {
+            return kept(r) ? x_row<E>(v, w.b, w.g, a.G, r0 + r) : nullptr;
+          };
+        };
+        fq.copy(row(a.q), a.D, l0);
+        fd.copy(row(a.dout), a.D, l0 + D0);
+      } else if (n < full) {
+        fq.start(first(a.q, r0), l0);
+        fd.start(first(a.dout, r0), l0 + D0);
       } else {
-        fq.template start<false>(first(a.q, r0), rhi - r0, l0);
-        fd.template start<false>(first(a.dout, r0), rhi - r0, l0 + D0);
+        fq.start_kept(first(a.q, r0), kept, l0);
+        fd.start_kept(first(a.dout, r0), kept, l0 + D0);
       }
     };
     feed(0);
@@ -1316,25 +1333,13 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
         const int r0 = rlo + (n + 3) * RT;
         const uint32_t l0 = ((n + 3) & 3) * C::TILE;
         stats(r0, l0);
-        fq.template start<true>(first(a.q, r0), RT, l0);
-        fd.template start<true>(first(a.dout, r0), RT, l0 + D0);
+        fq.start(first(a.q, r0), l0);
+        fd.start(first(a.dout, r0), l0 + D0);
       } else {
-        if (a.fast_q && n >= 0 && n + 2 < full)
+        if (a.fast_q && n >= 0 && n + 2 < np)
           ring_barrier<2 * F::N + 2 * STATS>();
         else
           ring_barrier<0>();
-        const int t0 = rlo + (n + 1) * RT;
-        if (t0 < rhi && t0 + RT > rhi) {
-          auto gone = [&](int r) { return t0 + r >= rhi; };
-          const uint32_t l0 = ((n + 1) & 3) * C::TILE;
-          fq.drop(gone, l0);
-          fd.drop(gone, l0 + D0);
-          if (threadIdx.x < RT && gone(threadIdx.x)) {
-            lds_stf(l0 + L0 + 4 * threadIdx.x, INFINITY);
-            lds_stf(l0 + T0 + 4 * threadIdx.x, 0.f);
-          }
-          __syncthreads();
-        }
         if (n >= 0) feed(n + 3);
       }
     };
@@ -1451,7 +1456,7 @@ inline XPlan x_plan(const XArgs& a, int type, int what) {
       break;
   }
   const long long blocks = p.tiles * heads;
-  const int each = type == 1 ? 64 : 256, most = (stream + each - 1) / each;
+  const int each = type == 1 ? 32 : 256, most = (stream + each - 1) / each;
   const long long want = blocks >= (own <= 32 ? 256 : 96) ? 1 : (255 + blocks) / blocks;
   p.splits = (int)(want < most ? want : most);
   return p;
