@@ -556,6 +556,80 @@ def test_token_steps_against_whole():
         within(whole[:, i:i + 1], want["o"], tol["o"], "whole")
 
 
+def module_reference(m, x, y, x_pos, y_pos, y_lens, y_mask):
+    """models.fusion_nets.CrossAttention in 64 bits on the CPU."""
+    w = {n: p.detach().double().cpu().requires_grad_() for n, p in m.named_parameters()}
+    x, y = (t.detach().double().cpu().requires_grad_() for t in (x, y))
+
+    def lin(t, n):
+        return t @ w[n + ".weight"].T + w[n + ".bias"]
+
+    def norm(t, g, pos):
+        t = t / torch.sqrt((t * t).mean(-1, keepdim=True) + m.eps) * g
+        if m.rope is None:
+            return t
+        r, n = m.rope, m.rope.dim // 2
+        f = r.base ** (-(torch.arange(n) % (n // r.axes)).double() / (n // r.axes))
+        a = pos.cpu().double().view(-1, r.axes).repeat_interleave(n // r.axes, -1) * f
+        c, s = torch.cos(a)[:, None], torch.sin(a)[:, None]
+        a, b = t[..., :n], t[..., n:2 * n]
+        return torch.cat([a * c - b * s, b * c + a * s, t[..., 2 * n:]], -1)
+    q = norm(lin(x, "query_proj").unflatten(-1, (m.heads, -1)), w["query_norm"], x_pos)
+    k, v = lin(y, "kv_proj").unflatten(-1, (2, m.kv_heads, -1)).unbind(2)
+    k = norm(k, w["key_norm"], y_pos)
+    k, v = (t.repeat_interleave(m.heads // m.kv_heads, 2) for t in (k, v))
+    score = torch.einsum("bihd,bjhd->bhij", q, k) / math.sqrt(m.head_dim)
+    keep = torch.arange(y.shape[1]) < y_lens.cpu()[:, None]
+    keep = (keep & y_mask.cpu())[:, None, None]
+    p = torch.softmax(score.masked_fill(~keep, -math.inf), -1)
+    o = torch.einsum("bhij,bjhd->bihd", p, v).flatten(-2)
+    return lin(o, "out_proj"), w, x, y
+
+
+@pytest.mark.parametrize("mode,bound", [("fp32", 1e-4), ("bf16", 3e-2), ("fp16", 3e-2)])
+def test_cross_attention_module(mode, bound):
+    """The module against 64 bits, forward and all gradients.  Bounds on the
+    relative 2-norm: fp32 projections carry 16-bit pairs, 2^-17 per operand
+    and element, of sums of up to 256 terms, through five products and their
+    derivatives; bf16 projections and operands round ten times by 2^-9 (the
+    softmax's derivative up to doubles what it is given): 20 2^-9 = 0.04 if
+    all of it added up, 0.015 as a root of squares."""
+    from text_guided_face_recognition_amd.models.fusion_nets import CrossAttention, set_precision
+    torch.manual_seed(5)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    rope = K.Rope(32, axes=2)
+    m = set_precision(CrossAttention(256, 192, heads=8, kv_heads=4, rope=rope).cuda(), mode)
+    with torch.no_grad():
+        m.query_norm.add_(0.2 * torch.randn_like(m.query_norm))
+        m.key_norm.add_(0.2 * torch.randn_like(m.key_norm))
+    x, y = randn(g, 3, 196, 256, dtype=F32), randn(g, 3, 29, 192, dtype=F32)
+    x.requires_grad_()
+    y.requires_grad_()
+    pos = (K.grid_positions(14, 14), torch.stack([torch.arange(29), torch.zeros(29)], 1).long()
+           .cuda())
+    lens = torch.tensor([29, 11, 1], device="cuda")
+    mask = torch.rand(3, 29, generator=g, device="cuda") > 0.2
+    mask[:, 0] = True
+    do = randn(g, 3, 196, 256, dtype=F32)
+    o = m(x, y, *pos, y_lens=lens, y_mask=mask)
+    names, params = zip(*m.named_parameters())
+    grads = torch.autograd.grad(o, (x, y, *params), do)
+    want, w, xd, yd = module_reference(m, x, y, *pos, lens, mask)
+    ref = torch.autograd.grad(want, (xd, yd, *(w[n] for n in names)), do.double().cpu())
+    # (kv_proj.bias's key half: the scores do not depend on what all keys share
+    # except through the norm; it is a small gradient, held to the whole bias)
+    for n, a, b in zip(("o", "x", "y", *names), (o, *grads), (want, *ref)):
+        off = float((a.detach().double().cpu() - b.detach()).norm() / b.detach().norm())
+        assert off < bound, f"{n}: {off:.3g}"
+    # single tokens against the kept context: the same rows
+    with torch.no_grad():
+        ctx = m.context(y, pos[1])
+        step = m(x[:, 7:8], x_pos=pos[0][7:8], y_lens=lens, y_mask=mask, context=ctx)
+    assert float((step - o[:, 7:8]).norm() / o[:, 7:8].norm()) < bound
+    with pytest.raises(ValueError):
+        m(x)
+
+
 def test_second_derivatives_are_refused():
     q, k, v, do, _ = inputs(F32, 1, 3, 4, 2, 2, 8)
     q.requires_grad_()

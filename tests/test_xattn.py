@@ -163,3 +163,10 @@ def test_c_entries_check_arguments():
                       (14, 258), (10, None)):
         assert fwd(at, value) == 1001, (at, value)
     assert fwd(16, 3) == 1002 and fwd(17, 1) == 1002      # bf16 is not written as fp32
+
+
+def test_module_refuses():
+    from text_guided_face_recognition_amd.models.fusion_nets import CrossAttention
+    for kw in (dict(channel_dim=30, heads=4), dict(channel_dim=32, heads=4, kv_heads=3)):
+        with pytest.raises(ValueError):
+            CrossAttention(**kw)

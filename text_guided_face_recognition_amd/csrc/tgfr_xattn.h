@@ -60,6 +60,7 @@ struct XArgs {
   int B, Tq, Tk, H, Hk, G, D, R;   // R = Tq G
   int splits, tiles;
   int fast_k, fast_q;              // rows may be read as whole aligned chunks, tile by tile
+  uint32_t per_g;                  // 2^32 / G, rounded up; 0 for G = 1
   float scale;
 };
 
@@ -90,6 +91,7 @@ struct XF16 {
 };
 struct XF32 {
   static constexpr int TYPE = 1, ES = 4;
+  static constexpr bool VEC = true;       // rows of whole 16-byte chunks
   using elem = float;
   static __device__ __forceinline__ f32x16 mma(uint4 a, uint4 b, f32x16 c) {
     c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
@@ -99,6 +101,10 @@ struct XF32 {
   }
   static __device__ __forceinline__ float val(float x) { return x; }
   static __device__ __forceinline__ float bits(float x) { return x; }
+};
+
+struct XF32Any : XF32 {
+  static constexpr bool VEC = false;
 };
 
 // 16 bytes at an address aligned to the element only (gfx950 reads and writes
@@ -306,33 +312,34 @@ struct LdsSrc {
 // fp32: straight from global memory.  Its matrix instructions take 8 times as
 // long per byte as bf16's, so cache reads hide behind them without a tile in
 // LDS; what counts is loads in flight, so a wave takes 64 columns (below).
-template <int DP>
+template <int DP, bool VEC, class At>
 struct MemSrc {
   __amdgpu_buffer_rsrc_t b;
-  uint32_t row, tro[16];
+  At at;
+  uint32_t row, live, tro[16];
   int lane, D;
   // the 32 rows whose first is at p (D: elements from there on); at(i): byte
   // offset of row i; bit i of `live`: row i exists (others are zeros)
-  template <class At>
-  __device__ __forceinline__ void begin(const void* p, At at, uint32_t live, int lane_, int D_) {
-    lane = lane_;
-    D = D_;
-    b = tile_rsrc(p);
-    const int r = lane & 31, h = lane >> 5;
+  __device__ __forceinline__ MemSrc(const void* p, At at_, uint32_t live_, int lane_, int D_)
+      : b(tile_rsrc(p)), at(at_), live(live_), lane(lane_), D(D_) {
+    const int r = lane & 31;
     row = (live >> r) & 1 ? at(r) : NONE;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int q = acc_row(i, h);
-      tro[i] = (live >> q) & 1 ? at(q) + 4 * r : NONE;
-    }
   }
   __device__ __forceinline__ uint4 rm(int j) const {
     const int d0 = 8 * j + 4 * (lane >> 5);
-    if ((D & 3) == 0) return buf16(b, d0 < D ? row + 4 * d0 : NONE);
+    if constexpr (VEC) return buf16(b, d0 < D ? row + 4 * d0 : NONE);
     return make_uint4(buf4(b, d0 < D ? row + 4 * d0 : NONE),
                       buf4(b, d0 + 1 < D ? row + 4 * d0 + 4 : NONE),
                       buf4(b, d0 + 2 < D ? row + 4 * d0 + 8 : NONE),
                       buf4(b, d0 + 3 < D ? row + 4 * d0 + 12 : NONE));
+  }
+  // before the first tr(): the rows' offsets, kept no longer than needed
+  __device__ __forceinline__ void open() {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int q = acc_row(i, lane >> 5);
+      tro[i] = (live >> q) & 1 ? at(q) + 4 * (lane & 31) : NONE;
+    }
   }
   __device__ __forceinline__ uint4 tr(int c, int db) const {
     const bool in = 32 * db + (lane & 31) < D;
@@ -341,6 +348,20 @@ struct MemSrc {
     for (int e = 0; e < 4; ++e) v[e] = buf4(b, in ? tro[4 * c + e] + 128 * db : NONE);
     return make_uint4(v[0], v[1], v[2], v[3]);
   }
+};
+// the same with all transposed operands read at once, before they are needed
+template <int DP, bool VEC, class At>
+struct HeldSrc : MemSrc<DP, VEC, At> {
+  using Src = MemSrc<DP, VEC, At>;
+  uint4 f[4 * (DP / 32)];
+  template <class... A>
+  __device__ __forceinline__ HeldSrc(A... a) : Src(a...) {
+    Src::open();
+#pragma unroll
+    for (int i = 0; i < 4 * (DP / 32); ++i)
+      f[i] = Src::tr(i / (DP / 32), i % (DP / 32));
+  }
+  __device__ __forceinline__ const uint4& tr(int c, int db) const { return f[c * (DP / 32) + db]; }
 };
 
 // ------------------------------------------------------------ shared parts ---
@@ -645,12 +666,17 @@ struct KeyStream {
         const int k0 = t0 + 32 * ws, j = k0 + (lane & 31);
         const uint32_t kb = (uint32_t)__ballot(j < khi && (!mask || mask[j]));
         if (DS == 1 && !kb) continue;
-        MemSrc<DH> ks, vs;
-        ks.begin(K + k0 * a.k.st, [&](int r) { return r * kst; }, kb, lane, a.D - ds * DH);
-        vs.begin(V + k0 * a.v.st, [&](int r) { return r * vst; }, kb, lane, a.D - ds * DH);
+        auto at_k = [=](int r) X_INLINE { return r * kst; };
+        auto at_v = [=](int r) X_INLINE { return r * vst; };
+        using V_ = decltype(at_v);
+        const int Dh = a.D - ds * DH;
+        MemSrc<DH, T::VEC, decltype(at_k)> ks(K + k0 * a.k.st, at_k, kb, lane, Dh);
+        using Src = std::conditional_t<FWD, HeldSrc<DH, T::VEC, V_>, MemSrc<DH, T::VEC, V_>>;
+        const Src vs(V + k0 * a.v.st, at_v, kb, lane, Dh);
         f32x16 sp[N];
         work(Yes{}, No{}, sp, ks, vs, sp, ks, vs);
         before(sp, kb);
+        if constexpr (!FWD) ks.open();
         work(No{}, Yes{}, sp, ks, vs, sp, ks, vs);
       }
     } else {
@@ -784,6 +810,7 @@ __device__ __forceinline__ void x_exchange(f32x16 (&s)[N], int group, int ds, in
           v += __builtin_bit_cast(f32x4, lds_ld16(base + x * 8192 + 4096 * n + 1024 * k));
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[n][4 * k + e] = v[e];
+        __builtin_amdgcn_sched_barrier(0);       // or all parts are in registers at once
       }
     turn ^= 1;
   }
@@ -796,9 +823,18 @@ struct Rows32 {
   uint4 f[I::NC];
   // p: the lane's row, or NULL for zeros, of D elements
   __device__ __forceinline__ void load(const typename T::elem* p, int D, int h) {
+    if (D % I::E == 0) {           // no branches, so all loads are in flight together
 #pragma unroll
-    for (int j = 0; j < I::NC; ++j)
-      f[j] = p && (2 * j + h) * I::E < D ? ld_chunk<T>(p, 2 * j + h, D) : zero16();
+      for (int j = 0; j < I::NC; ++j) {
+        const int d = (2 * j + h) * I::E;
+        f[j] = __builtin_bit_cast(
+            uint4, (u32x4) * (const u32x4_u*)(p && d < D ? (const void*)(p + d) : x_pad));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < I::NC; ++j)
+        f[j] = p && (2 * j + h) * I::E < D ? ld_chunk<T>(p, 2 * j + h, D) : zero16();
+    }
   }
   __device__ __forceinline__ const uint4& operator[](int j) const { return f[j]; }
 };
@@ -1008,12 +1044,13 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(c
   {
     const bool live = row < rows;
     const E* o = live ? x_row<E>(a.o, w.b, w.g, a.G, row) + ds * S::DH : nullptr;
+    Rows32<T, S::DH> of;
     qf.load(live ? x_row<E>(a.q, w.b, w.g, a.G, row) + ds * S::DH : nullptr, Dh, h);
     df.load(live ? x_row<E>(a.dout, w.b, w.g, a.G, row) + ds * S::DH : nullptr, Dh, h);
+    of.load(o, Dh, h);
 #pragma unroll
     for (int j = 0; j < I::NC; ++j) {
-      const uint4 dv = df[j];
-      const uint4 ov = o && (2 * j + h) * I::E < Dh ? ld_chunk<T>(o, 2 * j + h, Dh) : zero16();
+      const uint4 dv = df[j], ov = of[j];
       E x[I::E], y[I::E];
       __builtin_memcpy(x, &dv, 16);
       __builtin_memcpy(y, &ov, 16);
@@ -1237,9 +1274,9 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
   // byte offset of row i of a tile that begins with a token's first head
   auto in_tile = [&](const XView& v) {
     const uint32_t st = (uint32_t)v.st * T::ES, sh = (uint32_t)v.sh * T::ES;
-    const int G = a.G;
-    return [=](int i) -> uint32_t {
-      const uint32_t t = G == 1 ? i : (unsigned)i / (unsigned)G;
+    const uint32_t G = a.G, per = a.per_g, one = G == 1 ? ~0u : 0u;
+    return [=](uint32_t i) X_INLINE -> uint32_t {
+      const uint32_t t = __umulhi(i, per) + (i & one);       // i / G, i G < 2^32
       return t * st + (i - t * G) * sh;
     };
   };
@@ -1250,12 +1287,13 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
       if (DS == 1 && !live) continue;
       // offsets from the first row's token
       const int t0 = a.G == 1 ? r0 : (int)((unsigned)r0 / (unsigned)a.G), g0 = r0 - t0 * a.G;
-      MemSrc<DO> qs, os;
       const auto qo = in_tile(a.q), oo = in_tile(a.dout);
-      qs.begin(x_row<E>(a.q, w.b, w.g, a.G, t0 * a.G) + c0, [&](int i) { return qo(g0 + i); },
-               live, lane, a.D - c0);
-      os.begin(x_row<E>(a.dout, w.b, w.g, a.G, t0 * a.G) + c0, [&](int i) { return oo(g0 + i); },
-               live, lane, a.D - c0);
+      auto at_q = [=](int i) X_INLINE { return qo(g0 + i); };
+      auto at_o = [=](int i) X_INLINE { return oo(g0 + i); };
+      MemSrc<DO, T::VEC, decltype(at_q)> qs(x_row<E>(a.q, w.b, w.g, a.G, t0 * a.G) + c0, at_q, live,
+                                            lane, a.D - c0);
+      MemSrc<DO, T::VEC, decltype(at_o)> os(x_row<E>(a.dout, w.b, w.g, a.G, t0 * a.G) + c0, at_o,
+                                            live, lane, a.D - c0);
       auto stat = [&](const float* p, float none) {
         return [=](int k) {
           f32x4 v;
@@ -1270,6 +1308,8 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
       f32x16 sp[2];
       const auto lse = stat(a.lse, INFINITY), del = stat(a.delta, 0.f);
       work(Yes{}, No{}, sp, qs, os, lse, del, sp, qs, os);
+      qs.open();
+      os.open();
       work(No{}, Yes{}, sp, qs, os, lse, del, sp, qs, os);
     }
   } else {
@@ -1457,7 +1497,8 @@ inline XPlan x_plan(const XArgs& a, int type, int what) {
   }
   const long long blocks = p.tiles * heads;
   const int each = type == 1 ? 32 : 256, most = (stream + each - 1) / each;
-  const long long want = blocks >= (own <= 32 ? 256 : 96) ? 1 : (255 + blocks) / blocks;
+  const int slots = type == 1 ? 512 : 256;            // blocks at once
+  const long long want = blocks >= (own <= 32 ? slots : 96) ? 1 : (slots - 1 + blocks) / blocks;
   p.splits = (int)(want < most ? want : most);
   return p;
 }
@@ -1486,7 +1527,7 @@ template <class T, int DP, int W>
 int x_states(const XArgs& a, void* stream) {
   constexpr int DS = x_columns(T::TYPE, X_DKV, DP), WS = 4 / DS / W;
   using C = DkvCfg<T, DP, W, WS, DS>;
-  constexpr int OCC = T::ES == 2 && DP <= 128 && C::FED <= 80 * 1024 ? 2 : 1;
+  constexpr int OCC = DP <= (T::ES == 4 ? 64 : 128) && C::FED <= 80 * 1024 ? 2 : 1;
   return x_go(xattn_dkv<T, DP, W, WS, DS, OCC>, a, a.splits > 1 ? C::LDS32 : C::LDS, C::NT, stream);
 }
 template <class T, int DP, int W>

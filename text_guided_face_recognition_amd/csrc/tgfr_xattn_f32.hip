@@ -3,6 +3,6 @@
 
 namespace tgfr {
 int xattn_run_f32(const XArgs& a, int what, void* stream) {
-  return x_by_width<XF32>(a, what, stream);
+  return a.D % 4 ? x_by_width<XF32Any>(a, what, stream) : x_by_width<XF32>(a, what, stream);
 }
 }  // namespace tgfr

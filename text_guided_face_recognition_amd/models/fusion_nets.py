@@ -15,7 +15,7 @@ import torch.nn.functional as F
 
 from .. import kernels as K
 
-__all__ = ["SelfAttention", "Working", "conv1x1"]
+__all__ = ["SelfAttention", "CrossAttention", "Working", "conv1x1"]
 
 
 def conv1x1(in_planes, out_planes):
@@ -82,6 +82,78 @@ class SelfAttention(nn.Module):
         y_cl = x_cl if y is x else _cl(y)
         o = self.forward_cl(x_cl, y_cl)
         return o.reshape(n, h, w, c).permute(0, 3, 1, 2)
+
+
+class CrossAttention(nn.Module):
+    """Attention of one side's tokens to the other side's states of another
+    length (SelfAttention.forward needs one H*W on both, fusion_nets.py:105):
+    regions reading a caption's words, words reading the regions, or single
+    tokens against states that are kept.
+
+    `heads` query heads on `kv_heads` key heads (default: as many) of
+    channel_dim / heads elements; queries and keys are RMS-normed per head and,
+    with `rope` (kernels.Rope), rotated by their positions in the same launch
+    (kernels.qk_norm_rope), then kernels.cross_attention; 1x1 projections
+    around them as in SelfAttention.  precision "fp32" runs the attention in
+    fp32, "bf16" / "fp16" on tensors of that type."""
+
+    def __init__(self, channel_dim, context_dim=None, heads=4, kv_heads=None, rope=None,
+                 eps=1e-6):
+        super().__init__()
+        kv_heads = heads if kv_heads is None else kv_heads
+        if channel_dim % heads or heads % kv_heads:
+            raise ValueError(f"{channel_dim} channels, {heads} heads on {kv_heads} key heads")
+        self.heads, self.kv_heads = heads, kv_heads
+        self.head_dim = channel_dim // heads
+        kv = 2 * kv_heads * self.head_dim
+        self.query_proj = nn.Linear(channel_dim, channel_dim)
+        self.kv_proj = nn.Linear(channel_dim if context_dim is None else context_dim, kv)
+        self.out_proj = nn.Linear(channel_dim, channel_dim)
+        self.query_norm = nn.Parameter(torch.ones(self.head_dim))
+        self.key_norm = nn.Parameter(torch.ones(self.head_dim))
+        self.rope, self.eps = rope, eps
+        self.precision = "fp32"
+
+    def _dtype(self):
+        return {"fp32": torch.float32, "bf16": torch.bfloat16,
+                "fp16": torch.float16}[self.precision]
+
+    def _queries(self, x):
+        q = K.linear_rows(x, self.query_proj.weight, self.query_proj.bias, mode=self.precision)
+        return q.unflatten(-1, (self.heads, self.head_dim))
+
+    def _states(self, y):
+        kv = K.linear_rows(y, self.kv_proj.weight, self.kv_proj.bias, mode=self.precision)
+        return kv.unflatten(-1, (2, self.kv_heads, self.head_dim)).unbind(2)
+
+    def context(self, y, y_pos=None):
+        """The keys (normed, rotated) and values of y [N, T, context_dim], for
+        forward(..., context=...) of any number of later steps."""
+        k, v = self._states(y)
+        _, k = K.qk_norm_rope(None, k, None, self.key_norm, eps=self.eps, rope=self.rope,
+                              k_pos=y_pos, out_dtype=self._dtype())
+        return k, v.to(self._dtype())
+
+    def forward(self, x, y=None, x_pos=None, y_pos=None, x_lens=None, y_lens=None, y_mask=None,
+                context=None):
+        """x [N, Tx, channel_dim] reads y [N, Ty, context_dim] (or the kept
+        `context` of it) -> [N, Tx, channel_dim].  x_lens, y_lens [N]: tokens
+        of each sample; y_mask [N, Ty] (bool): False leaves a state out."""
+        if (y is None) == (context is None):
+            raise ValueError("either y or its context")
+        q, dtype = self._queries(x), self._dtype()
+        if context is None:
+            k, v = self._states(y)
+            q, k = K.qk_norm_rope(q, k, self.query_norm, self.key_norm, eps=self.eps,
+                                  rope=self.rope, q_pos=x_pos, k_pos=y_pos, out_dtype=dtype)
+            v = v.to(dtype)
+        else:
+            k, v = context
+            q, _ = K.qk_norm_rope(q, None, self.query_norm, None, eps=self.eps, rope=self.rope,
+                                  q_pos=x_pos, out_dtype=dtype)
+        o = K.cross_attention(q, k, v, q_lens=x_lens, kv_lens=y_lens, mask=y_mask)
+        return K.linear_rows(o.flatten(-2).float(), self.out_proj.weight, self.out_proj.bias,
+                             mode=self.precision)
 
 
 class Working(nn.Module):
