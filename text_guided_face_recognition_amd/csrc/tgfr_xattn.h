@@ -323,7 +323,9 @@ struct MemSrc {
   __device__ __forceinline__ MemSrc(const void* p, At at_, uint32_t live_, int lane_, int D_)
       : b(tile_rsrc(p)), at(at_), live(live_), lane(lane_), D(D_) {
     const int r = lane & 31;
-    row = (live >> r) & 1 ? at(r) : NONE;
+    row = at(r) | (~live >> r) << 31;
+    // opaque: offsets formed from it at each use, not kept over the loop
+    asm volatile("" : "+v"(row));
   }
   __device__ __forceinline__ uint4 rm(int j) const {
     const int d0 = 8 * j + 4 * (lane >> 5);
@@ -335,10 +337,11 @@ struct MemSrc {
   }
   // before the first tr(): the rows' offsets, kept no longer than needed
   __device__ __forceinline__ void open() {
+    asm volatile("" : "+v"(lane));
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int q = acc_row(i, lane >> 5);
-      tro[i] = (live >> q) & 1 ? at(q) + 4 * (lane & 31) : NONE;
+      tro[i] = (at(q) + 4 * (lane & 31)) | (~live >> q) << 31;     // no branch; at() < NONE
     }
   }
   __device__ __forceinline__ uint4 tr(int c, int db) const {
@@ -668,15 +671,17 @@ struct KeyStream {
         if (DS == 1 && !kb) continue;
         auto at_k = [=](int r) X_INLINE { return r * kst; };
         auto at_v = [=](int r) X_INLINE { return r * vst; };
+        using K_ = decltype(at_k);
         using V_ = decltype(at_v);
         const int Dh = a.D - ds * DH;
-        MemSrc<DH, T::VEC, decltype(at_k)> ks(K + k0 * a.k.st, at_k, kb, lane, Dh);
-        using Src = std::conditional_t<FWD, HeldSrc<DH, T::VEC, V_>, MemSrc<DH, T::VEC, V_>>;
-        const Src vs(V + k0 * a.v.st, at_v, kb, lane, Dh);
+        // the second product's operands (of V; dQ: of K) are read at the start
+        const std::conditional_t<FWD, MemSrc<DH, T::VEC, K_>, HeldSrc<DH, T::VEC, K_>> ks(
+            K + k0 * a.k.st, at_k, kb, lane, Dh);
+        const std::conditional_t<FWD, HeldSrc<DH, T::VEC, V_>, MemSrc<DH, T::VEC, V_>> vs(
+            V + k0 * a.v.st, at_v, kb, lane, Dh);
         f32x16 sp[N];
         work(Yes{}, No{}, sp, ks, vs, sp, ks, vs);
         before(sp, kb);
-        if constexpr (!FWD) ks.open();
         work(No{}, Yes{}, sp, ks, vs, sp, ks, vs);
       }
     } else {
@@ -823,7 +828,9 @@ struct Rows32 {
   uint4 f[I::NC];
   // p: the lane's row, or NULL for zeros, of D elements
   __device__ __forceinline__ void load(const typename T::elem* p, int D, int h) {
-    if (D % I::E == 0) {           // no branches, so all loads are in flight together
+    bool chunks = D % I::E == 0;
+    if constexpr (T::ES == 4) chunks = T::VEC;
+    if (chunks) {                  // no branches, so all loads are in flight together
 #pragma unroll
       for (int j = 0; j < I::NC; ++j) {
         const int d = (2 * j + h) * I::E;
@@ -1207,8 +1214,28 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
 
   const int c0 = C::MEM ? ds * DH : 0;         // first column of the operands
   Rows32<T, DO> kf, vf;
-  kf.load(kept ? x_key<E>(a.k, w.b, w.g, key) + c0 : nullptr, a.D - c0, h);
-  vf.load(kept ? x_key<E>(a.v, w.b, w.g, key) + c0 : nullptr, a.D - c0, h);
+  const uint32_t kept32 = (uint32_t)__ballot(kept);     // (both halves: the same states)
+  auto own = [&]() X_INLINE {
+    if constexpr (C::MEM) {
+      const uint32_t kst = (uint32_t)a.k.st * 4, vst = (uint32_t)a.v.st * 4;
+      auto at_k = [=](int r) X_INLINE { return r * kst; };
+      auto at_v = [=](int r) X_INLINE { return r * vst; };
+      const int k0 = key0 + 32 * wc;
+      const MemSrc<DO, T::VEC, decltype(at_k)> ks(x_key<E>(a.k, w.b, w.g, k0) + c0, at_k, kept32,
+                                                  lane, a.D - c0);
+      const MemSrc<DO, T::VEC, decltype(at_v)> vs(x_key<E>(a.v, w.b, w.g, k0) + c0, at_v, kept32,
+                                                  lane, a.D - c0);
+#pragma unroll
+      for (int j = 0; j < I::NC; ++j) {
+        kf.f[j] = ks.rm(j);
+        vf.f[j] = vs.rm(j);
+      }
+    } else {
+      kf.load(kept ? x_key<E>(a.k, w.b, w.g, key) : nullptr, a.D, h);
+      vf.load(kept ? x_key<E>(a.v, w.b, w.g, key) : nullptr, a.D, h);
+    }
+  };
+  if constexpr (!C::MEM) own();
   f32x16 dk[NB] = {}, dv[NB] = {};
   int turn = 0;
 
@@ -1300,14 +1327,18 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int i = 8 * k + 4 * h + e;
-            v[e] = i < n ? p[at + r0 + i] : none;
+            const float x = p[at + min(r0 + i, rhi - 1)];      // no branch
+            v[e] = i < n ? x : none;
           }
           return v;
         };
       };
+      asm volatile("" ::: "memory");
+      own();            // again for each piece: held over all, they would cost a wave per SIMD
       f32x16 sp[2];
       const auto lse = stat(a.lse, INFINITY), del = stat(a.delta, 0.f);
       work(Yes{}, No{}, sp, qs, os, lse, del, sp, qs, os);
+      __builtin_amdgcn_sched_barrier(0);
       qs.open();
       os.open();
       work(No{}, Yes{}, sp, qs, os, lse, del, sp, qs, os);
@@ -1527,7 +1558,7 @@ template <class T, int DP, int W>
 int x_states(const XArgs& a, void* stream) {
   constexpr int DS = x_columns(T::TYPE, X_DKV, DP), WS = 4 / DS / W;
   using C = DkvCfg<T, DP, W, WS, DS>;
-  constexpr int OCC = DP <= (T::ES == 4 ? 64 : 128) && C::FED <= 80 * 1024 ? 2 : 1;
+  constexpr int OCC = T::ES == 4 || (DP <= 128 && C::FED <= 80 * 1024) ? 2 : 1;
   return x_go(xattn_dkv<T, DP, W, WS, DS, OCC>, a, a.splits > 1 ? C::LDS32 : C::LDS, C::NT, stream);
 }
 template <class T, int DP, int W>
