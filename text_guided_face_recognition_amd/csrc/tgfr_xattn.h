@@ -217,11 +217,16 @@ __device__ __forceinline__ const void* scalar(const void* p) {
   const uint64_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)((uintptr_t)p >> 32));
   return (const void*)(lo | (hi << 32));
 }
-__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t to) {
+// (the lanes of `lanes` only, with no branch around it)
+__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t to,
+                                      uint64_t lanes) {
   const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_base() + to));
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off),
-               "s"(scalar(base)), "s"(m0)
-               : "memory", "m0");
+  uint64_t all;
+  asm volatile("s_mov_b64 %0, exec\n\ts_mov_b32 m0, %3\n\ts_and_b64 exec, exec, %4\n\t"
+               "global_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, %0"
+               : "=&s"(all)
+               : "v"(off), "s"(scalar(base)), "s"(m0), "s"(lanes)
+               : "memory", "m0", "scc");
 }
 __device__ __forceinline__ void dma4(const float* src, uint32_t to) {
   const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_base() + to));
@@ -239,8 +244,9 @@ struct Feed {
   using I = Img<T, DP>;
   static constexpr int N = ROWS * I::CPR / NT;
   static_assert(ROWS * I::CPR % NT == 0, "whole instructions");
-  uint32_t off[N];
-  bool whole;            // every chunk of the image is part of a row
+  uint32_t off[N], wave;     // (the wave's first place)
+  uint64_t lanes[N];         // whose chunks are part of a row
+  bool whole;                // all
 
   static __device__ __forceinline__ int row(int n) { return (threadIdx.x + NT * n) / I::CPR; }
   static __device__ __forceinline__ int chunk(int n) {
@@ -252,9 +258,12 @@ struct Feed {
   template <class At>
   __device__ __forceinline__ void init(At at, int D) {
     whole = D == DP;
+    wave = __builtin_amdgcn_readfirstlane(16 * (threadIdx.x & ~63u));
 #pragma unroll
-    for (int n = 0; n < N; ++n)
+    for (int n = 0; n < N; ++n) {
       off[n] = chunk(n) * I::E < D ? at(row(n)) + 16 * chunk(n) : NONE;
+      lanes[n] = __ballot(off[n] != NONE);
+    }
   }
   // columns past D, once: the feed leaves them alone
   __device__ __forceinline__ void clear(uint32_t base) const {
@@ -263,27 +272,20 @@ struct Feed {
     for (int n = 0; n < N; ++n)
       if (off[n] == NONE) lds_st16(base + place(n), zero16());
   }
-  // starts a whole tile whose first row is at p; N DMA instructions per wave
+  // starts a whole tile whose first row is at p; N DMA instructions per wave (an
+  // instruction covers whole rows: some lanes always take part)
   __device__ __forceinline__ void start(const void* p, uint32_t base) const {
-    const uint32_t to = base + 16 * (threadIdx.x & ~63u);
-    if (whole) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) dma16(p, off[n], to + 16 * NT * n);
-    } else {       // an instruction covers whole rows: some lanes always take part
-#pragma unroll
-      for (int n = 0; n < N; ++n)
-        if (off[n] != NONE) dma16(p, off[n], to + 16 * NT * n);
-    }
+    for (int n = 0; n < N; ++n) dma16(p, off[n], base + wave + 16 * NT * n, lanes[n]);
   }
   // the same with zeros for the rows that are not kept(row), which are not
   // read: their lanes fetch zeros from x_pad
   template <class Kept>
   __device__ __forceinline__ void start_kept(const void* p, Kept kept, uint32_t base) const {
-    const uint32_t to = base + 16 * (threadIdx.x & ~63u);
 #pragma unroll
     for (int n = 0; n < N; ++n)
       glds16(off[n] != NONE && kept(row(n)) ? (const char*)p + off[n] : (const char*)x_pad,
-             to + 16 * NT * n);
+             base + wave + 16 * NT * n);
   }
   // the same for rows at any alignment and of any length, through registers:
   // at(i) points to row i of the tile, or is NULL for zeros
@@ -546,30 +548,40 @@ constexpr int x_max(int a, int b) { return a > b ? a : b; }
 // columns' and its loads stay in flight.
 // One step in the order in which it is to run: RM products of the scores (of
 // the piece ahead), whose operands rm(i) are read AHEAD products early and
-// beside which beside(i) runs (the vector work of the current piece), then TR
-// products with operands tr(i).  (The compiler keeps this order where
-// accumulators fill the registers; written plainly, it read each operand right
-// before its product, and dK, dV took 2.5 times as long.)
-template <int RM, int TR, int AHEAD, class Rm, class Mma1, class Beside, class Between, class Tr,
-          class Mma2>
-__device__ __forceinline__ void x_step(Rm rm, Mma1 mma1, Beside beside, Between between, Tr tr,
-                                       Mma2 mma2) {
+// beside which beside(i) runs (the vector work of the current piece, after
+// early() has read what it needs), then TR products with operands tr(i).  KEEP
+// holds the compiler to this order.  Alone on its SIMD a wave needs that: the
+// compiler reads operands two at a time right before their products.  Two
+// waves fill each other's gaps, and their registers leave no room for it.
+template <int RM, int TR, int AHEAD, bool KEEP, class Rm, class Mma1, class Early, class Beside,
+          class Between, class Tr, class Mma2>
+__device__ __forceinline__ void x_step(Rm rm, Mma1 mma1, Early early, Beside beside,
+                                       Between between, Tr tr, Mma2 mma2) {
   uint4 f[AHEAD];
   auto load = [&](int i) X_INLINE { return i < RM ? rm(i) : tr(i - RM); };
+  auto keep = []() X_INLINE {
+    if constexpr (KEEP) __builtin_amdgcn_sched_barrier(0);
+  };
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i)
     if (i < RM + TR) f[i] = load(i);
+  keep();
+  early();
+  keep();
 #pragma unroll
   for (int i = 0; i < RM; ++i) {
     mma1(i, f[i % AHEAD]);
     if (i + AHEAD < RM + TR) f[i % AHEAD] = load(i + AHEAD);
     beside(i);
+    keep();
   }
   between();
+  keep();
 #pragma unroll
   for (int i = RM; i < RM + TR; ++i) {
     mma2(i - RM, f[i % AHEAD]);
     if (i + AHEAD < RM + TR) f[i % AHEAD] = load(i + AHEAD);
+    keep();
   }
 }
 struct XNone {
@@ -911,9 +923,10 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(
       l += sp[0][e];
     };
     if constexpr (A) next[0] = f32x16{};
-    x_step<RM, TR, S::AHEAD>(
+    x_step<RM, TR, S::AHEAD, OCC == 1>(
         [&](int i) X_INLINE { return kn.rm(i); },
         [&](int i, uint4 f) X_INLINE { next[0] = T::mma(f, qf[i], next[0]); },
+        []() X_INLINE {},
         [&](int i) X_INLINE {
           if constexpr (B)
 #pragma unroll
@@ -1093,11 +1106,12 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(c
       constexpr int RM = A ? 2 * I::NC : 0, TR = B && P ? I::NPF * NB : 0;
       uint4 p[I::NPF];
       if constexpr (A) next[0] = next[1] = f32x16{};
-      x_step<RM, TR, S::AHEAD>(
+      x_step<RM, TR, S::AHEAD, OCC == 1>(
           [&](int i) X_INLINE { return i & 1 ? vn.rm(i / 2) : kn.rm(i / 2); },
           [&](int i, uint4 f) X_INLINE {
             next[i & 1] = T::mma(f, i & 1 ? df[i / 2] : qf[i / 2], next[i & 1]);
           },
+          []() X_INLINE {},
           [&](int i) X_INLINE {
             if constexpr (B)
 #pragma unroll
@@ -1169,7 +1183,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(c
 // products where 4 would do).
 template <class T, int DP, int WC, int WS, int DS>
 struct DkvCfg {
-  static constexpr int NT = 64 * WC * WS * DS, RT = 32 * WS, AHEAD = T::ES == 4 ? 8 : 4;
+  static constexpr int NT = 64 * WC * WS * DS, RT = 32 * WS, AHEAD = T::ES == 4 ? 8 : DP == 128 ? 6 : 4;
   static constexpr bool MEM = T::ES == 4;
   static constexpr int TILE = MEM ? 0 : 2 * Img<T, DP>::bytes(RT) + 8 * RT;   // Q, dO, L, delta
   static constexpr int FED = MEM ? (DS > 1 ? 2 * 8192 * WC * WS * DS : 0) : 4 * TILE;
@@ -1247,29 +1261,37 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
     constexpr int RM = A ? 2 * I::NC : 0, TR = B ? 2 * I::NPF * NB : 0;
     const int b0 = C::MEM ? 0 : ds * NB;
     f32x4 L[4], t[4];
-    if constexpr (B)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        L[k] = lse(k);
-        t[k] = del(k);
-      }
     uint4 p[I::NPF], g[I::NPF];
     auto element = [&](int i) X_INLINE {
       sp[0][i] = __builtin_amdgcn_exp2f(fmaf(sp[0][i], c2, -L[i / 4][i % 4]));
       sp[1][i] = sp[0][i] * (sp[1][i] - t[i / 4][i % 4]);
       if constexpr (std::is_same<T, XF16>::value) sp[1][i] *= down;
     };
+    auto pack = [&](int c) X_INLINE {
+      p[c] = I::pack(sp[0], c);
+      g[c] = I::pack(sp[1], c);
+    };
     if constexpr (A) next[0] = next[1] = f32x16{};
-    x_step<RM, TR, C::AHEAD>(
+    x_step<RM, TR, C::AHEAD, OCC == 1>(
         [&](int i) X_INLINE { return i & 1 ? on.rm(i / 2) : qn.rm(i / 2); },
         [&](int i, uint4 f) X_INLINE {
           next[i & 1] = T::mma(f, i & 1 ? vf[i / 2] : kf[i / 2], next[i & 1]);
         },
-        [&](int i) X_INLINE {
+        [&]() X_INLINE {
           if constexpr (B)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              L[k] = lse(k);
+              t[k] = del(k);
+            }
+        },
+        [&](int i) X_INLINE {
+          if constexpr (B) {
+            if (i == RM / 2 && I::NPF == 2) pack(0);
 #pragma unroll
             for (int e = 0; e < 16; ++e)
               if (e * RM / 16 == i) element(e);
+          }
         },
         [&]() X_INLINE {
           if constexpr (B) {
@@ -1277,10 +1299,7 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
 #pragma unroll
               for (int e = 0; e < 16; ++e) element(e);
 #pragma unroll
-            for (int c = 0; c < I::NPF; ++c) {
-              p[c] = I::pack(sp[0], c);
-              g[c] = I::pack(sp[1], c);
-            }
+            for (int c = A && I::NPF == 2 ? 1 : 0; c < I::NPF; ++c) pack(c);
           }
         },
         [&](int i) X_INLINE {
@@ -1346,7 +1365,7 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
   } else {
     constexpr uint32_t D0 = I::bytes(RT), L0 = 2 * D0, T0 = L0 + 4 * RT;
     using F = Feed<T, DP, RT, C::NT>;
-    constexpr int STATS = (RT + 63) / 64;             // instructions for L, delta each
+    constexpr int STATS = 2 * RT / 64;                // instructions for L and delta
     F fq, fd;
     fq.init(in_tile(a.q), a.D);
     fd.init(in_tile(a.dout), a.D);
@@ -1356,16 +1375,22 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
       fd.clear(i * C::TILE + D0);
     }
     const int np = (rhi - rlo + RT - 1) / RT, full = (rhi - rlo) / RT;
-    // L and delta of a tile; every wave fetches them (the same values to the
-    // same places), so that all waves count the same instructions
-    auto stats = [&](int r0, uint32_t l0) X_INLINE {
+    // L and delta of a tile, one after the other; every wave fetches them (the
+    // same values to the same places), so that all count the same instructions
+    const float* stat_at[STATS];
+#pragma unroll
+    for (int i = 0; i < STATS; ++i) {
+      const int j = 64 * i + lane;
+      stat_at[i] = (j < RT ? a.lse : a.delta) + at + rlo + j % RT;
+    }
+    auto stats = [&](int n, uint32_t l0, auto plain) X_INLINE {
 #pragma unroll
       for (int i = 0; i < STATS; ++i) {
-        const int r = r0 + 64 * i + lane;
-        if (64 * i + lane < RT) {
-          dma4(r < rhi ? a.lse + at + r : x_pad + 4, l0 + L0 + 256 * i);
-          dma4(r < rhi ? a.delta + at + r : x_pad, l0 + T0 + 256 * i);
-        }
+        const int j = 64 * i + lane;
+        const float* p = stat_at[i] + n * RT;
+        if constexpr (!plain.value)
+          if (rlo + n * RT + j % RT >= rhi) p = j < RT ? x_pad + 4 : x_pad;
+        dma4(p, l0 + L0 + 256 * i);
       }
     };
     // a tile's first row, where G, a power of two, divides RT
@@ -1377,7 +1402,7 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
       const int r0 = rlo + n * RT;
       const uint32_t l0 = (n & 3) * C::TILE;
       if (n >= np) return;
-      stats(r0, l0);
+      stats(n, l0, No{});
       auto kept = [&](int r) X_INLINE { return r0 + r < rhi; };
       if (!a.fast_q) {
         auto row = [&](const XView& v) X_INLINE {
@@ -1400,15 +1425,15 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
     feed(2);
     auto wait = [&](int n, auto plain) X_INLINE {
       if constexpr (plain.value) {
-        ring_barrier<2 * F::N + 2 * STATS>();
+        ring_barrier<2 * F::N + STATS>();
         const int r0 = rlo + (n + 3) * RT;
         const uint32_t l0 = ((n + 3) & 3) * C::TILE;
-        stats(r0, l0);
+        stats(n + 3, l0, Yes{});
         fq.start(first(a.q, r0), l0);
         fd.start(first(a.dout, r0), l0 + D0);
       } else {
         if (a.fast_q && n >= 0 && n + 2 < np)
-          ring_barrier<2 * F::N + 2 * STATS>();
+          ring_barrier<2 * F::N + STATS>();
         else
           ring_barrier<0>();
         if (n >= 0) feed(n + 3);
@@ -1500,11 +1525,11 @@ struct XPlan {
 // each took 0.6 of the time of one wave of 32, whose registers leave no room
 // for a second).
 constexpr int x_columns(int type, int what, int dp) {
-  return type == 1 ? dp / 64 : what == X_DKV && dp >= 128 ? 2 : 1;
+  return type == 1 ? dp / 64 : what == X_DKV && dp > 128 ? 2 : 1;
 }
 // Least waves that own rows (states): the rings of fewer would pass the LDS.
 constexpr int x_least(int type, int what, int dp) {
-  return type == 1 || dp <= 64 ? 1 : what == X_DKV ? dp / 128 : dp == 128 ? 2 : 4;
+  return type == 1 || dp <= 64 ? 1 : what == X_DKV ? 2 : dp == 128 ? 2 : 4;
 }
 // The split of one kernel's work.  `own` rows (dK, dV: states) belong to the
 // waves, the others are streamed.  A block's four waves (or those that the
@@ -1558,7 +1583,7 @@ template <class T, int DP, int W>
 int x_states(const XArgs& a, void* stream) {
   constexpr int DS = x_columns(T::TYPE, X_DKV, DP), WS = 4 / DS / W;
   using C = DkvCfg<T, DP, W, WS, DS>;
-  constexpr int OCC = T::ES == 4 || (DP <= 128 && C::FED <= 80 * 1024) ? 2 : 1;
+  constexpr int OCC = T::ES == 4 || (DP <= 64 && C::FED <= 80 * 1024) ? 2 : 1;
   return x_go(xattn_dkv<T, DP, W, WS, DS, OCC>, a, a.splits > 1 ? C::LDS32 : C::LDS, C::NT, stream);
 }
 template <class T, int DP, int W>
