@@ -6,6 +6,8 @@
 //
 // Holds no kernels: bind() takes the addresses of the C entries (tgfr.h) from
 // the library that the process has loaded.
+#include <limits>
+
 #include <ATen/Functions.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -246,8 +248,12 @@ py::object cross_attention(py::handle hq, py::handle hk, py::handle hv, py::hand
     bad_value("mask must be a bool tensor [", a.b, ", ", a.tk, "]");
   on_device(a.q, {{"k", a.k}, {"v", a.v}, {"q_lens", a.q_lens}, {"kv_lens", a.kv_lens},
                   {"mask", a.mask}});
-  if (a.q_lens.defined()) a.q_lens = a.q_lens.to(at::kInt).contiguous();
-  if (a.kv_lens.defined()) a.kv_lens = a.kv_lens.to(at::kInt).contiguous();
+  for (at::Tensor* lens : {&a.q_lens, &a.kv_lens})
+    if (lens->defined()) {
+      if (lens->scalar_type() == at::kLong)             // (must not wrap)
+        *lens = lens->clamp(-1, std::numeric_limits<int>::max()).to(at::kInt);
+      *lens = lens->contiguous();
+    }
   if (a.mask.defined()) a.mask = dense(a.mask);
   const bool grad = at::GradMode::is_enabled() &&
                     (a.q.requires_grad() || a.k.requires_grad() || a.v.requires_grad());

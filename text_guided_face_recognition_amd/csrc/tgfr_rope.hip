@@ -18,7 +18,10 @@
 // load, LPR lanes per head.  A wave takes one token, or as many as fill it
 // where heads are few; its lanes form the sines of the tokens' pairs once, each
 // another one, and share them through LDS (formed by each lane for itself,
-// they took more vector instructions than all the rest).
+// they took more vector instructions than all the rest).  4 x 4096 tokens of 32
+// + 8 heads of 128, bf16: 75 us, 4.5 TB/s (a copy: 4.7).  Backward of 2 x 4096 of
+// them: 70 us, 3.6 TB/s, three streams and the partial sums of dw, whose second
+// launch takes 5 us.
 #include "tgfr_common.h"
 
 using namespace tgfr;
@@ -79,10 +82,6 @@ struct __attribute__((packed, aligned(sizeof(E)))) Pack {
 
 // Where a lane's V pairs lie.  Chunked loads need them in one piece: the
 // elements a0 .. and b0 .. (or 2 V from a0 on, interleaved).
-struct Place {
-  int p0;        // first pair; pairs past D / 2 do not exist
-  int a0, b0;
-};
 __device__ __forceinline__ int n_first(const NArgs& a, int p) {
   if (a.interleaved) return 2 * p;
   return p < a.R / 2 ? p : a.R + (p - a.R / 2);

@@ -20,7 +20,7 @@
 // order; its A operand is read from LDS transposed in that order.
 //
 // fp32 runs on v_mfma_f32_32x32x2_f32 (every product and sum in 32 bits).
-// bf16 / fp16 round P and dS to the type as MFMA operands (2^-9 / 2^-12
+// bf16 / fp16 round P and dS to the type as MFMA operands (2^-8 / 2^-11
 // relative, of the size of the one rounding of the result); sums, statistics
 // and accumulators are fp32.
 //
@@ -205,9 +205,6 @@ __device__ __forceinline__ uint32_t buf4(__amdgpu_buffer_rsrc_t r, uint32_t off)
   return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
 }
 
-// 16 bytes per lane from a scalar base + lane offset (4 from an address) straight
-// to LDS byte `to` (wave-uniform) + 16 (4) * lane.  Inline asm, so that the compiler sees no
-// LDS write pending on the memory counter; the kernels wait by count (glds16).
 // zeros for places that are not read, then the statistics of such rows (log
 // sum +infinity: probability 0; delta 0)
 static __device__ const float x_pad[8] __attribute__((aligned(16))) = {
@@ -217,7 +214,13 @@ __device__ __forceinline__ const void* scalar(const void* p) {
   const uint64_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)((uintptr_t)p >> 32));
   return (const void*)(lo | (hi << 32));
 }
-// (the lanes of `lanes` only, with no branch around it)
+// 16 bytes per lane of `lanes` from a scalar base + lane offset (4 of every lane
+// from an address) straight to LDS byte `to` (wave-uniform) + 16 (4) * lane.
+// Inline asm, so that the compiler sees no LDS write pending on the memory
+// counter; the kernels wait by count (glds16).  Lanes are chosen by exec, not by
+// branches: around those the accumulators were moved from register to register
+// (dK and dV of 4 x 1024 rows, 16 heads of 128 on 4, on 1500 states: 149 us
+// against 161).
 __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t to,
                                       uint64_t lanes) {
   const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_base() + to));
@@ -246,7 +249,6 @@ struct Feed {
   static_assert(ROWS * I::CPR % NT == 0, "whole instructions");
   uint32_t off[N], wave;     // (the wave's first place)
   uint64_t lanes[N];         // whose chunks are part of a row
-  bool whole;                // all
 
   static __device__ __forceinline__ int row(int n) { return (threadIdx.x + NT * n) / I::CPR; }
   static __device__ __forceinline__ int chunk(int n) {
@@ -257,7 +259,6 @@ struct Feed {
   // at(i): byte offset of row i from the tile's first
   template <class At>
   __device__ __forceinline__ void init(At at, int D) {
-    whole = D == DP;
     wave = __builtin_amdgcn_readfirstlane(16 * (threadIdx.x & ~63u));
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -267,7 +268,6 @@ struct Feed {
   }
   // columns past D, once: the feed leaves them alone
   __device__ __forceinline__ void clear(uint32_t base) const {
-    if (whole) return;
 #pragma unroll
     for (int n = 0; n < N; ++n)
       if (off[n] == NONE) lds_st16(base + place(n), zero16());
@@ -543,16 +543,19 @@ constexpr int x_max(int a, int b) { return a > b ? a : b; }
 //
 // fp32 with more than 64 columns: DS waves take 64 columns each of Q, K, V and
 // the result.  Each forms its part of the scores, the parts are exchanged
-// through LDS and summed by all in one order (1/8 of the time of the products
-// they belong to), so a wave's operands and accumulators are a quarter of 256
-// columns' and its loads stay in flight.
+// through LDS and summed by all in one order, so a wave's operands and
+// accumulators are a quarter of 256 columns' and its loads stay in flight.
 // One step in the order in which it is to run: RM products of the scores (of
 // the piece ahead), whose operands rm(i) are read AHEAD products early and
 // beside which beside(i) runs (the vector work of the current piece, after
 // early() has read what it needs), then TR products with operands tr(i).  KEEP
-// holds the compiler to this order.  Alone on its SIMD a wave needs that: the
-// compiler reads operands two at a time right before their products.  Two
-// waves fill each other's gaps, and their registers leave no room for it.
+// holds the compiler to this order, which else reads operands two at a time
+// right before their products.  Alone on its SIMD a wave of dK, dV needs that
+// (167 -> 161 us at 4 x 1024 rows, 16 heads of 128 on 4, on 1500 states; 212 ->
+// 177 us at 4 x 1024 x 1024, 8 heads of 256 on 2), and dQ of up to 128 columns
+// gains a little (34 -> 33 us at 3 x 333 x 777, 6 heads of 80 on 3); the
+// forward (31 -> 32) and dQ of 256 columns (85 -> 88) do not, and where two waves
+// share a SIMD it costs registers that they lack.
 template <int RM, int TR, int AHEAD, bool KEEP, class Rm, class Mma1, class Early, class Beside,
           class Between, class Tr, class Mma2>
 __device__ __forceinline__ void x_step(Rm rm, Mma1 mma1, Early early, Beside beside,
@@ -867,6 +870,11 @@ __device__ __forceinline__ void x_mask(f32x16& s, uint32_t kb, int h) {
 }
 
 // ------------------------------------------------------------------ forward ---
+// 4 x 2048 rows of 16 heads of 128 on 4 x 4096 states of 4, bf16: 261 us, 1050
+// TFLOP/s, bound by the matrix units (a library product of 8192^3: 1172).  One
+// token, 16 samples, 32 heads on 8, up to 8192 states: 72 us, 4.8 TB/s, bound by
+// reading K and V.  fp32, 64 x 30 rows on 196 states of 256: 15 us, bound by the
+// latency of its 7 splits' few pieces.
 template <class T, int DP, int WR, int WS, int DS, int OCC>
 __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(const XArgs a) {
   using S = KeyStream<T, DP, WR, WS, DS, true>;
@@ -923,7 +931,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(
       l += sp[0][e];
     };
     if constexpr (A) next[0] = f32x16{};
-    x_step<RM, TR, S::AHEAD, OCC == 1>(
+    x_step<RM, TR, S::AHEAD, false>(
         [&](int i) X_INLINE { return kn.rm(i); },
         [&](int i, uint4 f) X_INLINE { next[0] = T::mma(f, qf[i], next[0]); },
         []() X_INLINE {},
@@ -988,7 +996,8 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(
 }
 
 // Joins the splits of the forward: a block per row, 256 / W threads sharing
-// each of the W >= D columns.
+// each of the W >= D columns.  Bound by its launch and one read of the parts:
+// 1920 rows of 256 in 7 splits, fp32, 8 us; 512 rows of 128 in 4 splits, 5 us.
 template <class T, int W>
 __global__ __launch_bounds__(256) void xattn_fwd_join(const XArgs a) {
   using E = typename T::elem;
@@ -1040,7 +1049,9 @@ __device__ __forceinline__ float x_down(float amax) {
 }
 
 // dQ of WR * 32 rows, streaming K and V; also delta (and the rows' |dO|) for
-// xattn_dkv, which runs after it.
+// xattn_dkv, which runs after it.  4 x 2048 rows on 2048 states, 16 heads of 128,
+// bf16: 194 us, 1061 TFLOP/s, bound by the matrix units.  fp32, 64 x 30 rows on
+// 196 states of 256: 20 us.
 template <class T, int DP, int WR, int WS, int DS, int OCC>
 __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(const XArgs a) {
   using S = KeyStream<T, DP, WR, WS, DS, false>;
@@ -1106,7 +1117,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(c
       constexpr int RM = A ? 2 * I::NC : 0, TR = B && P ? I::NPF * NB : 0;
       uint4 p[I::NPF];
       if constexpr (A) next[0] = next[1] = f32x16{};
-      x_step<RM, TR, S::AHEAD, OCC == 1>(
+      x_step<RM, TR, S::AHEAD, OCC == 1 && DP <= 128>(
           [&](int i) X_INLINE { return i & 1 ? vn.rm(i / 2) : kn.rm(i / 2); },
           [&](int i, uint4 f) X_INLINE {
             next[i & 1] = T::mma(f, i & 1 ? df[i / 2] : qf[i / 2], next[i & 1]);
@@ -1178,12 +1189,18 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(c
 
 // dK and dV of WC * 32 states, streaming Q and dO, 32 WS rows at a time; WS
 // waves share the states and take different rows, DS waves the columns of the
-// results: of fp32 as above, of 16-bit types because both accumulators are too
-// large for one wave's registers (each of the two forms all of the scores, 6
-// products where 4 would do).
+// results: of fp32 as above, of 16-bit types past 128 columns because both
+// accumulators are too large for one wave's registers (each of the two forms
+// all of the scores, 6 products where 4 would do).
+//
+// 4 x 2048 rows on 2048 states, 16 heads of 128, bf16: 290 us, 946 TFLOP/s.
+// A wave of 128 columns is alone on its SIMD and issues 320 instructions a
+// piece in the time of 32 matrix instructions and half as long again: bound by
+// issue.  fp32, 64 x 30 rows on 196 states of 256: 26 us, 65 TFLOP/s.
 template <class T, int DP, int WC, int WS, int DS>
 struct DkvCfg {
-  static constexpr int NT = 64 * WC * WS * DS, RT = 32 * WS, AHEAD = T::ES == 4 ? 8 : DP == 128 ? 6 : 4;
+  static constexpr int NT = 64 * WC * WS * DS, RT = 32 * WS;
+  static constexpr int AHEAD = T::ES == 4 ? 8 : DP == 128 ? 6 : 4;
   static constexpr bool MEM = T::ES == 4;
   static constexpr int TILE = MEM ? 0 : 2 * Img<T, DP>::bytes(RT) + 8 * RT;   // Q, dO, L, delta
   static constexpr int FED = MEM ? (DS > 1 ? 2 * 8192 * WC * WS * DS : 0) : 4 * TILE;
@@ -1340,22 +1357,20 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
                                             lane, a.D - c0);
       MemSrc<DO, T::VEC, decltype(at_o)> os(x_row<E>(a.dout, w.b, w.g, a.G, t0 * a.G) + c0, at_o,
                                             live, lane, a.D - c0);
-      auto stat = [&](const float* p, float none) {
-        return [=](int k) {
-          f32x4 v;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = 8 * k + 4 * h + e;
-            const float x = p[at + min(r0 + i, rhi - 1)];      // no branch
-            v[e] = i < n ? x : none;
-          }
-          return v;
-        };
-      };
       asm volatile("" ::: "memory");
       own();            // again for each piece: held over all, they would cost a wave per SIMD
       f32x16 sp[2];
-      const auto lse = stat(a.lse, INFINITY), del = stat(a.delta, 0.f);
+      f32x4 L[4], delta[4];            // read before the products that they wait beside
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = acc_row(i, h);
+        const long long j = at + min(r0 + r, rhi - 1);         // no branch
+        const float x = a.lse[j], y = a.delta[j];
+        L[i / 4][i % 4] = r < n ? x : INFINITY;
+        delta[i / 4][i % 4] = r < n ? y : 0.f;
+      }
+      auto lse = [&](int k) X_INLINE { return L[k]; };
+      auto del = [&](int k) X_INLINE { return delta[k]; };
       work(Yes{}, No{}, sp, qs, os, lse, del, sp, qs, os);
       __builtin_amdgcn_sched_barrier(0);
       qs.open();
@@ -1521,9 +1536,9 @@ struct XPlan {
   int waves, tiles, splits;      // waves that own rows (dK, dV: states), 32 each
 };
 // Waves along the columns: fp32 64 columns each; dK, dV of 16-bit types two
-// waves from 128 columns on (at 128, two waves per SIMD of 24 products a piece
-// each took 0.6 of the time of one wave of 32, whose registers leave no room
-// for a second).
+// waves past 128 columns (at 128, one wave of 32 products a piece, alone on its
+// SIMD, took 149 us where two of 24 took 166: 4 x 1024 rows, 16 heads on 4, on
+// 1500 states).
 constexpr int x_columns(int type, int what, int dp) {
   return type == 1 ? dp / 64 : what == X_DKV && dp > 128 ? 2 : 1;
 }
