@@ -88,6 +88,25 @@ def test_qk_norm_rope_refuses_widening():
         K.qk_norm_rope(**norm_args(dtype=torch.bfloat16), out_dtype=torch.float32)
 
 
+def test_qk_norm_rope_refuses_a_changed_rope():
+    """Sizes that a Rope's steps do not fit are refused, never read past."""
+    for name, value in (("dim", 12), ("dim", 10), ("axes", 3), ("turn", torch.zeros(8)),
+                        ("turn", torch.zeros(16).long()[::2])):
+        rope = K.Rope(16, device="cpu")
+        setattr(rope, name, value)
+        pos = dict(q_pos=torch.zeros(5, 3).long(), k_pos=torch.zeros(7, 3).long()) \
+            if rope.axes == 3 else {}
+        with pytest.raises(ValueError):
+            K.qk_norm_rope(**{**norm_args(), "rope": rope, **pos})
+
+
+def test_qk_norm_rope_refuses_too_many_tokens():
+    """Token numbers are 32-bit."""
+    x = torch.zeros(1, 1, 1, 16).expand(1, (1 << 30) + 1, 1, 16)
+    with pytest.raises(ValueError):
+        K.qk_norm_rope(x, None, torch.ones(16), None)
+
+
 @pytest.mark.parametrize("kw", [dict(dim=0), dict(dim=15), dict(dim=6, axes=2),
                                 dict(dim=8, axes=0), dict(dim=8, base=0.5),
                                 dict(dim=8, base=float("inf"))])

@@ -441,11 +441,15 @@ py::object qk_norm_rope(py::handle hq, py::handle hk, py::handle hwq, py::handle
   if (a.pos[0].defined() && a.pos[1].defined() &&
       a.pos[0].scalar_type() != a.pos[1].scalar_type())
     bad_type("q_pos and k_pos need one type");
-  constexpr int64_t most = 1LL << 31;
+  constexpr int64_t most = 1LL << 30;
   for (const Tensor& t : a.x)
-    if (t.defined() && (t.size(0) >= most || t.size(1) >= most || t.size(2) >= most ||
-                        t.size(0) * t.size(1) >= most))
-      bad_value("at most 2^31 - 1 tokens");
+    if (t.defined() && (t.size(0) > most || t.size(1) > most || t.size(2) > most ||
+                        t.size(0) * t.size(1) > most))
+      bad_value("at most 2^30 tokens, and heads of one");
+  if (a.turn.defined() &&
+      (a.turn.scalar_type() != at::kLong || a.turn.dim() != 1 || !a.turn.is_contiguous() ||
+       rot < 2 || axes < 1 || rot % (2 * axes) || a.turn.size(0) != rot / 2))
+    bad_value("rope does not hold ", rot, " / 2 steps over ", axes, " axes");
   on_device(x, {{"k", a.x[1]}, {"q_weight", a.w[0]}, {"k_weight", a.w[1]}, {"q_pos", a.pos[0]},
                 {"k_pos", a.pos[1]}, {"rope", a.turn}});
   bool grad = false;
