@@ -181,7 +181,7 @@ def test_attention_lengths_and_masks(dtype, size):
 # chunk holds, over several splits; many heads on one
 WIDE = [(70, 20, 40, 2, 1, 64), (130, 3, 70, 2, 2, 128), (1, 2, 40000, 2, 1, 64),
         (1, 5, 3000, 3, 1, 128), (1, 2, 3001, 2, 1, 5), (2, 3, 200, 64, 1, 64),
-        (1, 600, 70, 48, 2, 72)]
+        (1, 600, 70, 48, 2, 72), (12, 2, 700, 16, 8, 128)]
 
 
 @pytest.mark.parametrize("dtype", [BF, F16, F32], ids=["bf16", "fp16", "fp32"])

@@ -1544,34 +1544,47 @@ struct XPlan {
 constexpr int x_columns(int type, int what, int dp) {
   return type == 1 ? dp / 64 : what == X_DKV && dp > 128 ? 2 : 1;
 }
-// Least waves that own rows (states): the rings of fewer would pass the LDS.
+// Least waves that own rows (states): the rings of fewer would pass the LDS, or
+// of 64 columns leave a CU one block instead of two (4 x 5 x 1500, 12 heads,
+// masked: 13.3 us against 15.0 at each one's best splits).
 constexpr int x_least(int type, int what, int dp) {
-  return type == 1 || dp <= 64 ? 1 : what == X_DKV ? 2 : dp == 128 ? 2 : 4;
+  if (type == 1 || (dp == 64 && what == X_DKV)) return 1;
+  return dp <= 128 || what == X_DKV ? 2 : 4;
 }
 // The split of one kernel's work.  `own` rows (dK, dV: states) belong to the
 // waves, the others are streamed.  A block's four waves (or those that the
 // columns leave) own 32 rows each while that gives every CU a block; below,
 // two or all of them share rows and take different parts of the stream, where
 // that has a piece of 32 for each (1 x 2048 x 2048 of 8 heads on one: 38 us
-// against 48; 8 x 64 x 512, 8 heads of 64: 10.0 against 12.8).  What still
-// leaves CUs without a block splits the stream over blocks, 256 items or more
-// each, whose results a second launch joins (17 tokens of 8 heads on 8192
-// states: 32 us against 114; not at 99 blocks: 22 both ways).
+// against 48; 8 x 64 x 512, 8 heads of 64: 10.0 against 12.8); not for a few rows
+// of 128 columns under a mask, whose steps take longer than their tiles, where
+// the splits fill the card by themselves, two blocks to a CU (16 x 1 x 8192, 32
+// heads on 8: 101 us against 142; without a mask 84 against 77).  What still leaves
+// CUs without a block splits the stream over blocks, 128 items (fp32: 64) or
+// more each and no more blocks than run at once; a second launch joins them
+// (17 tokens of 8 heads on 8192 states: 32 us against 114; not at 99 blocks: 22
+// both ways; 4 x 5 x 1500, 12 heads of 64, masked: 14.4 us in one round of 384 or
+// more blocks, 21.7 in one and an eighth; 64 x 30 x 196 of 256, fp32: 21.2 us by 4
+// splits, 23.0 by 7).
 inline XPlan x_plan(const XArgs& a, int type, int what) {
   const int own = what == X_DKV ? a.Tk : a.R, stream = what == X_DKV ? a.R : a.Tk;
   const long long heads = (long long)a.B * a.Hk;
   const int dp = a.D <= 64 ? 64 : a.D <= 128 ? 128 : 256, all = 4 / x_columns(type, what, dp);
+  const bool masked = a.mask && dp == 128 && what != X_DKV;
   XPlan p;
   for (p.waves = all;; p.waves /= 2) {
     p.tiles = (own + 32 * p.waves - 1) / (32 * p.waves);
     if (p.waves == x_least(type, what, dp) || p.tiles * heads >= 256 ||
-        stream <= 32 * (all / p.waves))
+        stream <= 32 * (all / p.waves) || (masked && own <= 32 && heads >= 96))
       break;
   }
   const long long blocks = p.tiles * heads;
-  const int each = type == 1 ? 32 : 256, most = (stream + each - 1) / each;
-  const int slots = type == 1 ? 512 : 256;            // blocks at once
-  const long long want = blocks >= (own <= 32 ? slots : 96) ? 1 : (slots - 1 + blocks) / blocks;
+  const int each = type == 1 ? 64 : 128, most = (stream + each - 1) / each;
+  // blocks at once: two per CU where their rings leave room
+  const bool two = type == 1 || (dp == 64 && p.waves > 1) ||
+                   (dp == 128 && p.waves == 4 && what != X_DKV);
+  const int slots = two ? 512 : 256;
+  const long long want = blocks >= (own <= 32 ? slots : 96) ? 1 : slots / blocks;
   p.splits = (int)(want < most ? want : most);
   return p;
 }

@@ -1,4 +1,6 @@
 // C entries of cross attention (kernels: tgfr_xattn.h, one file per type).
+#include <algorithm>
+
 #include "tgfr_xattn.h"
 
 using namespace tgfr;
@@ -28,6 +30,8 @@ int x_shape(XArgs& a, int type, int B, int Tq, int Tk, int H, int Hk, int D) {
   a.per_g = a.G == 1 ? 0 : (uint32_t)(((1ULL << 32) + a.G - 1) / a.G);
   return 0;
 }
+
+const uint8_t* const ANY_MASK = (const uint8_t*)1;    // (for the plan, never read)
 
 long long x_part(const XArgs& a, int type, int what) {
   const bool kv = what == X_DKV;
@@ -66,12 +70,16 @@ int tgfr_cross_attention_ws(int B, int Tq, int Tk, int H, int Hk, int D, int typ
   XArgs a{};
   if (!floats) return 1001;
   if (const int e = x_shape(a, type, B, Tq, Tk, H, Hk, D)) return e;
-  if (!backward) {
-    *floats = x_part(a, type, X_FWD);
-    return 0;
+  // enough with a mask and without
+  long long n = 0;
+  for (const uint8_t* mask : {(const uint8_t*)nullptr, ANY_MASK}) {
+    a.mask = mask;
+    if (!backward)
+      n = std::max(n, x_part(a, type, X_FWD));
+    else
+      n = std::max({n, x_part(a, type, X_DQ), x_part(a, type, X_DKV)});
   }
-  const long long q = x_part(a, type, X_DQ), kv = x_part(a, type, X_DKV);
-  *floats = 2LL * B * Hk * a.R + (q > kv ? q : kv);
+  *floats = n + (backward ? 2LL * B * Hk * a.R : 0);
   return 0;
 }
 
@@ -83,6 +91,7 @@ int tgfr_cross_attention_fwd(const void* q, const void* k, const void* v, void* 
   XArgs a{};
   if (const int e = x_shape(a, type, B, Tq, Tk, H, Hk, D)) return e;
   if (!q || !k || !v || !o || !strides || !(scale > 0.f)) return 1001;
+  a.mask = mask;
   const long long n = x_part(a, type, X_FWD);
   if (n && !ws) return 1001;
   a.q = view(q, strides);
@@ -92,7 +101,6 @@ int tgfr_cross_attention_fwd(const void* q, const void* k, const void* v, void* 
   if (const int e = x_reading(a, type)) return e;
   a.q_lens = q_lens;
   a.kv_lens = kv_lens;
-  a.mask = mask;
   a.mask_sb = mask_sb;
   a.scale = scale;
   a.lse = lse;
