@@ -876,7 +876,7 @@ __device__ __forceinline__ void x_mask(f32x16& s, uint32_t kb, int h) {
 // TFLOP/s, bound by the matrix units (a library product of 8192^3: 1172).  One
 // token, 16 samples, 32 heads on 8, up to 8192 states: 72 us, 4.8 TB/s, bound by
 // reading K and V.  fp32, 64 x 30 rows on 196 states of 256: 15 us, bound by the
-// latency of its 7 splits' few pieces.
+// latency of its 4 splits' two pieces.
 template <class T, int DP, int WR, int WS, int DS, int OCC>
 __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(const XArgs a) {
   using S = KeyStream<T, DP, WR, WS, DS, true>;
@@ -999,7 +999,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(
 
 // Joins the splits of the forward: a block per row, 256 / W threads sharing
 // each of the W >= D columns.  Bound by its launch and one read of the parts:
-// 1920 rows of 256 in 7 splits, fp32, 8 us; 512 rows of 128 in 4 splits, 5 us.
+// 1920 rows of 256 in 4 splits, fp32, 6 us; 512 rows of 128 in 2 splits, 5 us.
 template <class T, int W>
 __global__ __launch_bounds__(256) void xattn_fwd_join(const XArgs a) {
   using E = typename T::elem;
@@ -1563,8 +1563,8 @@ constexpr int x_least(int type, int what, int dp) {
 // CUs without a block splits the stream over blocks, 128 items (fp32: 64) or
 // more each and no more blocks than run at once; a second launch joins them
 // (17 tokens of 8 heads on 8192 states: 32 us against 114; not at 99 blocks: 22
-// both ways; 4 x 5 x 1500, 12 heads of 64, masked: 14.4 us in one round of 384 or
-// more blocks, 21.7 in one and an eighth; 64 x 30 x 196 of 256, fp32: 21.2 us by 4
+// both ways; 4 x 5 x 1500, 12 heads of 64, masked: 14.4 us in one round of 480
+// blocks, 21.7 in one and an eighth of 256; 64 x 30 x 196 of 256, fp32: 21.2 us by 4
 // splits, 23.0 by 7).
 inline XPlan x_plan(const XArgs& a, int type, int what) {
   const int own = what == X_DKV ? a.Tk : a.R, stream = what == X_DKV ? a.R : a.Tk;
@@ -1581,8 +1581,10 @@ inline XPlan x_plan(const XArgs& a, int type, int what) {
   const long long blocks = p.tiles * heads;
   const int each = type == 1 ? 64 : 128, most = (stream + each - 1) / each;
   // blocks at once: two per CU where their rings leave room
-  const bool two = type == 1 || (dp == 64 && p.waves > 1) ||
-                   (dp == 128 && p.waves == 4 && what != X_DKV);
+  // (dK, dV join twice as much: 64 x 196 rows on 32 states, 4 heads of 64, 14 us
+  // unsplit, 16 + 11 in two)
+  const bool two = type == 1 || (what != X_DKV && ((dp == 64 && p.waves > 1) ||
+                                                   (dp == 128 && p.waves == 4)));
   const int slots = two ? 512 : 256;
   const long long want = blocks >= (own <= 32 ? slots : 96) ? 1 : slots / blocks;
   p.splits = (int)(want < most ? want : most);
