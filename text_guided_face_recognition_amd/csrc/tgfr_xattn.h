@@ -220,13 +220,15 @@ __device__ __forceinline__ const void* scalar(const void* p) {
 // counter; the kernels wait by count (glds16).  Lanes are chosen by exec, not by
 // branches: around those the accumulators were moved from register to register
 // (dK and dV of 4 x 1024 rows, 16 heads of 128 on 4, on 1500 states: 149 us
-// against 161).
+// against 161).  The s_nop completes the five wait states that a scalar register
+// written by a vector instruction (readfirstlane: the base) needs before a
+// memory instruction reads it, which the compiler cannot see to in here.
 __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t to,
                                       uint64_t lanes) {
   const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_base() + to));
   uint64_t all;
   asm volatile("s_mov_b64 %0, exec\n\ts_mov_b32 m0, %3\n\ts_and_b64 exec, exec, %4\n\t"
-               "global_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, %0"
+               "s_nop 1\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, %0"
                : "=&s"(all)
                : "v"(off), "s"(scalar(base)), "s"(m0), "s"(lanes)
                : "memory", "m0", "scc");
