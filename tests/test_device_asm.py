@@ -19,6 +19,7 @@ WAIT = 5
 # the assembly
 PROBE = {
     "dma16": ("tgfr_xattn.h", "tgfr::dma16(p[t], o[t], 0, tgfr::x_probe_lanes(o[t]));"),
+    "glds16s": ("tgfr_common.h", "tgfr::glds16s(p[t], o[t], 0);"),
 }
 
 
