@@ -107,6 +107,27 @@ def test_qk_norm_rope_refuses_too_many_tokens():
         K.qk_norm_rope(x, None, torch.ones(16), None)
 
 
+@pytest.mark.parametrize("which", ["q", "k", "v"])
+def test_cross_attention_refuses_tangents(which):
+    """Forward mode: no derivative is given, and none is dropped in silence."""
+    x = dict(zip("qkv", qkv()))
+    with torch.autograd.forward_ad.dual_level():
+        x[which] = torch.autograd.forward_ad.make_dual(x[which], torch.ones_like(x[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            K.cross_attention(**x)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            K.cross_attention(**x)
+
+
+@pytest.mark.parametrize("which", ["q", "k", "q_weight", "k_weight"])
+def test_qk_norm_rope_refuses_tangents(which):
+    x = norm_args()
+    with torch.autograd.forward_ad.dual_level():
+        x[which] = torch.autograd.forward_ad.make_dual(x[which], torch.ones_like(x[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            K.qk_norm_rope(**x)
+
+
 @pytest.mark.parametrize("kw", [dict(dim=0), dict(dim=15), dict(dim=6, axes=2),
                                 dict(dim=8, axes=0), dict(dim=8, base=0.5),
                                 dict(dim=8, base=float("inf"))])

@@ -9,6 +9,7 @@
 #include <limits>
 
 #include <ATen/Functions.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
@@ -115,6 +116,14 @@ void on_device(const Tensor& x, std::initializer_list<std::pair<const char*, Ten
 void no_second_derivative(const char* name) {
   if (at::GradMode::is_enabled())
     throw std::runtime_error(text("the backward of ", name, " is not differentiable"));
+}
+
+// A node is made by requires_grad alone: a tangent would be lost in silence.
+void no_tangent(const char* name, std::initializer_list<Tensor> inputs) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor& t : inputs)
+    if (t.defined() && t._fw_grad(0).defined())
+      throw std::runtime_error(text(name, " has no forward-mode derivative"));
 }
 
 // --------------------------------------------------------- cross attention ---
@@ -246,6 +255,7 @@ py::object cross_attention(py::handle hq, py::handle hk, py::handle hv, py::hand
   if (a.mask.defined() && (a.mask.scalar_type() != at::kBool || a.mask.dim() != 2 ||
                            a.mask.size(0) != a.b || a.mask.size(1) != a.tk))
     bad_value("mask must be a bool tensor [", a.b, ", ", a.tk, "]");
+  no_tangent("cross_attention", {a.q, a.k, a.v});
   on_device(a.q, {{"k", a.k}, {"v", a.v}, {"q_lens", a.q_lens}, {"kv_lens", a.kv_lens},
                   {"mask", a.mask}});
   for (at::Tensor* lens : {&a.q_lens, &a.kv_lens})
@@ -450,6 +460,7 @@ py::object qk_norm_rope(py::handle hq, py::handle hk, py::handle hwq, py::handle
       (a.turn.scalar_type() != at::kLong || a.turn.dim() != 1 || !a.turn.is_contiguous() ||
        rot < 2 || axes < 1 || rot % (2 * axes) || a.turn.size(0) != rot / 2))
     bad_value("rope does not hold ", rot, " / 2 steps over ", axes, " axes");
+  no_tangent("qk_norm_rope", {a.x[0], a.x[1], a.w[0], a.w[1]});
   on_device(x, {{"k", a.x[1]}, {"q_weight", a.w[0]}, {"k_weight", a.w[1]}, {"q_pos", a.pos[0]},
                 {"k_pos", a.pos[1]}, {"rope", a.turn}});
   bool grad = false;
