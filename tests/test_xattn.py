@@ -128,6 +128,15 @@ def test_qk_norm_rope_refuses_tangents(which):
             K.qk_norm_rope(**x)
 
 
+def test_tracing_is_refused():
+    """A trace would hold the output's allocation and not the kernel."""
+    n = norm_args()
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda *x: K.cross_attention(*x), qkv())
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda q, w: K.qk_norm_rope(q, None, w, None)[0], (n["q"], n["q_weight"]))
+
+
 @pytest.mark.parametrize("kw", [dict(dim=0), dict(dim=15), dict(dim=6, axes=2),
                                 dict(dim=8, axes=0), dict(dim=8, base=0.5),
                                 dict(dim=8, base=float("inf"))])

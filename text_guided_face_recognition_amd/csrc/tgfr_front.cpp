@@ -15,6 +15,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
@@ -126,6 +127,12 @@ void no_tangent(const char* name, std::initializer_list<Tensor> inputs) {
       throw std::runtime_error(text(name, " has no forward-mode derivative"));
 }
 
+// A trace would record the output's allocation and not the kernel.
+void no_trace(const char* name) {
+  if (torch::jit::tracer::isTracing())
+    throw std::runtime_error(text(name, " cannot be traced"));
+}
+
 // --------------------------------------------------------- cross attention ---
 struct Attn {
   Tensor q, k, v, q_lens, kv_lens, mask;
@@ -224,6 +231,7 @@ Tensor lens_given(py::handle h, const char* name, int64_t n) {
 
 py::object cross_attention(py::handle hq, py::handle hk, py::handle hv, py::handle hscale,
                            py::handle hql, py::handle hkl, py::handle hmask) {
+  no_trace("cross_attention");
   Attn a;
   a.q = given(hq, "q"), a.k = given(hk, "k"), a.v = given(hv, "v");
   for (const auto& x : {std::make_pair("q", &a.q), std::make_pair("k", &a.k),
@@ -415,6 +423,7 @@ void positions(const char* name, Norm& a, int i, bool rope) {
 py::object qk_norm_rope(py::handle hq, py::handle hk, py::handle hwq, py::handle hwk, double eps,
                         py::handle hturn, int64_t rot, int64_t axes, bool interleaved,
                         py::handle hqp, py::handle hkp, py::handle hout) {
+  no_trace("qk_norm_rope");
   Norm a;
   a.x[0] = given(hq, "q"), a.x[1] = given(hk, "k");
   a.turn = given(hturn, "rope");

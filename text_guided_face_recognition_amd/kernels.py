@@ -2241,8 +2241,8 @@ def cross_attention(q, k, v, scale=None, q_lens=None, kv_lens=None, mask=None):
     give equal bits.  Only enqueues work on the current stream of q's device:
     can be captured into a HIP graph, a backward together with its forward
     (autograd runs a backward on its forward's stream, so one whose forward
-    ran eagerly does not belong into a capture).  Second derivatives and
-    forward-mode tangents are refused."""
+    ran eagerly does not belong into a capture).  Second derivatives,
+    forward-mode tangents and torch.jit.trace are refused."""
     return _hip.front().cross_attention(q, k, v, scale, q_lens, kv_lens, mask)
 
 
@@ -2294,8 +2294,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, eps=1e-6, rope=None, q_pos=None, k_po
     Positions: int32 or int64, any size, [T] or [B, T] (with more rope axes
     [T, axes] or [B, T, axes]); None: 0 .. T - 1.  D even, at most 256.  Equal
     calls give equal bits, and the call can be captured into a HIP graph (a
-    backward together with its forward).  Second derivatives and forward-mode
-    tangents are refused."""
+    backward together with its forward).  Second derivatives, forward-mode
+    tangents and torch.jit.trace are refused."""
     if rope is None:
         return _hip.front().qk_norm_rope(q, k, q_weight, k_weight, eps, None, 0, 1, False, q_pos,
                                          k_pos, out_dtype)
