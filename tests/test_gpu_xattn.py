@@ -6,12 +6,14 @@ make: u is half a step of the tensors' type (the result; P and dS as matrix
 operands), e the fp32 arithmetic: a sum of n products is off by at most
 (n + 8) 2^-24 of the sum of their magnitudes, and a probability by twice the
 error of its score (as an exponent) and the error of its row's sum."""
+import ctypes
 import math
 from decimal import Decimal, getcontext
 
 import pytest
 import torch
 
+from text_guided_face_recognition_amd import _hip
 from text_guided_face_recognition_amd import kernels as K
 
 pytestmark = pytest.mark.gpu
@@ -671,3 +673,108 @@ def test_second_derivatives_are_refused():
     for o in (K.cross_attention(q, k, v), K.qk_norm_rope(q, None, w, None)[0]):
         with pytest.raises(RuntimeError, match="not differentiable"):
             torch.autograd.grad(o.sum(), q, create_graph=True)
+
+
+def plan_floats(size, dtype, backward):
+    """Workspace of a call: what splits and their joins need."""
+    b, tq, tk, h, hk, d = size
+    n = ctypes.c_longlong(0)
+    code = {BF: 0, F32: 1, F16: 2}[dtype]
+    assert _hip.lib().tgfr_cross_attention_ws(b, tq, tk, h, hk, d, code, backward,
+                                              ctypes.byref(n)) == 0
+    return n.value
+
+
+# One share of the stream long enough for the loops of whole tiles, four at a
+# time and twice over, with a tail: 11 tiles or more for each block of each
+# kernel.  128 columns by four waves and by two, 64 by two (dK, dV one), 256.
+DEEP = [(12, 300, 400, 16, 8, 128), (3, 400, 750, 8, 4, 128), (3, 750, 750, 8, 4, 64),
+        (4, 400, 400, 8, 4, 256)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("size", DEEP, ids=["x".join(map(str, s)) for s in DEEP])
+def test_attention_loops_of_whole_tiles(dtype, size):
+    b, tq, tk, h, hk, d = size
+    assert plan_floats(size, dtype, 0) == 0                       # nothing is split
+    assert plan_floats(size, dtype, 1) <= 2 * b * h * tq          # (statistics alone)
+    *x, g = inputs(dtype, *size)
+    check(*x)
+    q_lens = torch.randint(tq * 3 // 4, tq + 1, (b,), generator=g, device="cuda")
+    kv_lens = torch.randint(tk * 3 // 4, tk + 1, (b,), generator=g, device="cuda")
+    check(*x, q_lens=q_lens, kv_lens=kv_lens)
+    mask = torch.rand(b, tk, generator=g, device="cuda") > 0.15
+    check(*x, kv_lens=kv_lens, mask=mask)
+
+
+def shifted(x, by):
+    """The same values in rows 2 elements longer, from element `by` on: any
+    row may begin at any multiple of four bytes."""
+    b, t, h, d = x.shape
+    wide = x.new_full((b * t * (h * d + 2) + 16,), float("nan"))
+    y = wide[by:by + b * t * (h * d + 2)].view(b, t, h * d + 2)[..., :h * d].view(b, t, h, d)
+    return y.copy_(x)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("size", [(2, 130, 300, 4, 2, 64), (3, 400, 750, 8, 4, 128),
+                                  (2, 9, 2100, 8, 2, 80), (1, 70, 90, 2, 2, 256)],
+                         ids=["64", "128", "few", "256"])
+def test_attention_rows_at_four_bytes(dtype, size):
+    """Whole chunks of 16 bytes from rows that begin at four."""
+    *x, g = inputs(dtype, *size)
+    o, grads = check(*x)
+    mask = torch.rand(size[0], size[2], generator=g, device="cuda") > 0.15
+    om, grads_m = check(*x, mask=mask)
+    y = [shifted(t, by) for t, by in zip(x, (2, 6, 10, 4))]
+    for t in y:
+        assert t.data_ptr() % 16 and t.data_ptr() % 4 == 0 and t.stride(1) % 8
+    for m, want in ((None, (o, *grads)), (mask, (om, *grads_m))):
+        leaves = [t.detach().requires_grad_() for t in y[:3]]
+        got = K.cross_attention(*leaves, mask=m)
+        for a, c in zip((got, *torch.autograd.grad(got, leaves, y[3])), want):
+            assert torch.equal(a, c)
+
+
+def close_in_norm(got, want, names, bound):
+    for n, x in zip(names, got):
+        assert bool(torch.isfinite(x).all()), f"{n} is not finite"
+        off = float((x.double() - want[n]).norm() / want[n].norm())
+        assert off <= bound, f"{n}: {off:.3g} of {bound:.3g}"
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32], ids=["bf16", "fp16", "fp32"])
+def test_attention_past_one_reading_of_the_mask(dtype):
+    """More states than one reading of the mask holds (32768), not split, so
+    that one block's loop begins again: running maximum, sum and accumulators
+    carried over.  Held in the 2-norm, where independent roundings of at most
+    u (uniform: u / sqrt 3) of the terms of a sum and of its result make up
+    0.9 u, and dS doubles its share of them: 2 u, and 1e-4 for fp32 sums of
+    33000 terms (2^-24 sqrt(33000) = 1.1e-5 and the scores' 4 (40 + 8) 2^-24
+    = 1.2e-5).  The states past 32768 alone are 8 % of the norm."""
+    size = b, tq, tk, h, hk, d = (1, 2112, 33000, 3, 3, 32)
+    *x, g = inputs(dtype, *size)
+    assert plan_floats(size, dtype, 0) == 0
+    bound = 2 * half_step(dtype) + 1e-4
+    mask = torch.rand(b, tk, generator=g, device="cuda") > 0.15
+    for lens, m in ((None, None), (None, mask), (32769, mask), (32768, mask)):
+        kv_lens = None if lens is None else torch.tensor([lens], device="cuda")
+        leaves = [t.detach().requires_grad_() for t in x[:3]]
+        o = K.cross_attention(*leaves, kv_lens=kv_lens, mask=m)
+        grads = torch.autograd.grad(o, leaves, x[3])
+        want, _ = formula(*x, d ** -0.5, keep_of(b, tq, tk, None, kv_lens, m))
+        close_in_norm((o.detach(), *grads), want, ("o", "dq", "dk", "dv"), bound)
+        del want
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32], ids=["bf16", "fp16", "fp32"])
+def test_attention_long_states_lose_no_split(dtype):
+    """Splits of few states each, held in the 2-norm: any one of them is 5 % of
+    it or more (40000 states in at most 313 splits: sqrt(1 / 313))."""
+    *x, _ = inputs(dtype, 1, 2, 40000, 2, 1, 64)
+    leaves = [t.detach().requires_grad_() for t in x[:3]]
+    o = K.cross_attention(*leaves)
+    grads = torch.autograd.grad(o, leaves, x[3])
+    want, _ = formula(*x, 0.125, keep_of(1, 2, 40000))
+    close_in_norm((o.detach(), *grads), want, ("o", "dq", "dk", "dv"),
+                  2 * half_step(dtype) + 1e-4)
