@@ -697,7 +697,7 @@ DEEP = [(12, 300, 400, 16, 8, 128), (3, 400, 750, 8, 4, 128), (3, 750, 750, 8, 4
 def test_attention_loops_of_whole_tiles(dtype, size):
     b, tq, tk, h, hk, d = size
     assert plan_floats(size, dtype, 0) == 0                       # nothing is split
-    assert plan_floats(size, dtype, 1) <= 2 * b * h * tq          # (statistics alone)
+    assert plan_floats(size, dtype, 1) < d * min(b * h * tq, b * hk * tk)   # (no parts)
     *x, g = inputs(dtype, *size)
     check(*x)
     q_lens = torch.randint(tq * 3 // 4, tq + 1, (b,), generator=g, device="cuda")
@@ -778,3 +778,35 @@ def test_attention_long_states_lose_no_split(dtype):
     want, _ = formula(*x, 0.125, keep_of(1, 2, 40000))
     close_in_norm((o.detach(), *grads), want, ("o", "dq", "dk", "dv"),
                   2 * half_step(dtype) + 1e-4)
+
+
+@pytest.mark.parametrize("size", [(1, 4, 2, 1, 1, 256), (2, 70, 300, 4, 2, 128),
+                                  (1, 40, 3000, 2, 1, 64), (2, 200, 500, 4, 2, 256)],
+                         ids=["two", "tiles", "split", "wide"])
+@pytest.mark.parametrize("big,small", [(600.0, 2.0 ** -10), (2.0 ** 14, 2.0 ** -12),
+                                       (2.0 ** -12, 2.0 ** 10), (2.0 ** -6, 2.0 ** -8)])
+def test_attention_fp16_values_of_any_size(size, big, small):
+    """dS = P (dO.V - delta) grows with V as well as with dO: large values of
+    one sign against small gradients, and the other way round.  Beside the
+    bounds of all types dS may lose 2^-39 of 2 |dO| |V| of the row (dK: of the
+    head's largest) and of the largest state: half a step below fp16's range,
+    2^-25, where that bound of dS is held at 2^14 or more."""
+    b, tq, tk, h, hk, d = size
+    q, k, v, do, g = inputs(F16, *size)
+    sign = torch.where(torch.arange(tk, device="cuda") % 2 == 0, 1.0, -1.0).view(1, tk, 1, 1)
+    v = (sign * big * (1 + 0.1 * v.float().clamp(-3, 3))).to(F16)
+    do = (small * (1 + 0.1 * do.float().clamp(-3, 3))).to(F16)
+    scale = d ** -0.5
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = K.cross_attention(*leaves, scale=scale)
+    grads = torch.autograd.grad(o, leaves, do)
+    want, tol = formula(q, k, v, do, scale, keep_of(b, tq, tk))
+    dp = 2 * heads(do, h).norm(dim=-1, keepdim=True) * \
+        heads(v, h).norm(dim=-1).amax(-1)[..., None, None]
+    tol["dq"] = tol["dq"] + (scale * 2.0 ** -39 * dp * heads(k, h).abs().sum(
+        2, keepdim=True)).transpose(1, 2)
+    per_head = dp.view(b, hk, -1, 1).amax(2, keepdim=True)           # [B, Hk, 1, 1]
+    rows = heads(q, h).abs().sum(2).view(b, hk, -1, d).sum(2, keepdim=True)
+    tol["dk"] = tol["dk"] + (scale * 2.0 ** -39 * per_head * rows).transpose(1, 2)
+    for n, x in zip(("o", "dq", "dk", "dv"), (o.detach(), *grads)):
+        within(x, want[n], tol[n], n)

@@ -54,11 +54,12 @@ struct XArgs {
   long long mask_sb;
   float* lse;            // [B Hk][R]: log2 of the row's sum, in the log2 domain; +inf: none
   float* delta;          // [B Hk][R]
-  float* amax;           // [B Hk][R] largest |dO| of the row (fp16 only)
+  float* size;           // [B Hk][R] |dO| of the row (fp16 only)
+  float* vmax;           // [B Hk][chunks] squares of the largest |V| (fp16 only)
   float* part;           // partial results of the splits
   float* part_ml;        // forward: [split][B Hk][R][2] maximum and sum
   int B, Tq, Tk, H, Hk, G, D, R;   // R = Tq G
-  int splits, tiles;
+  int splits, tiles, chunks;
   int fast_k, fast_q;              // rows may be read as whole aligned chunks, tile by tile
   uint32_t per_g;                  // 2^32 / G, rounded up; 0 for G = 1
   float scale;
@@ -1040,19 +1041,71 @@ __global__ __launch_bounds__(256) void xattn_fwd_join(const XArgs a) {
 }
 
 // ----------------------------------------------------------------- backward ---
-// fp16 holds dS from 2^-24 to 2^16 only: dS is scaled by a power of two taken
-// from the largest |dO| (of the row for dQ, of all rows for dK, whose sum runs
-// over them), and the sum is scaled back in fp32.  bf16 and fp32 need none.
+// fp16 holds dS from 2^-24 to 2^16 only: dS is scaled by a power of two and the
+// sum scaled back in fp32.  |dP| and |delta| are at most |dO| |V| in the 2-norm, of
+// the row (for dK, whose sum runs over all rows, of the largest) and of the
+// largest kept state, so |dS| <= 2 |dO| |V| =: b as P <= 1.  The scale brings b to
+// [2^14, 2^15): nothing overflows, and dS keeps all of fp16's digits down to
+// 2^-28 b.  (Following the largest dP from piece to piece instead spares the
+// launch below, but costs registers: backward of 4 x 2048 rows on 2048 states,
+// 16 heads of 128, 710 us against 541.)  bf16 and fp32 need none.
 template <class T>
-__device__ __forceinline__ float x_down(float amax) {
-  if constexpr (std::is_same<T, XF16>::value) {
-    const uint32_t e = (__float_as_uint(amax) >> 23) & 255;
-    return e == 0 || e == 255 ? 1.f : __uint_as_float((254 - e) << 23);
+struct DownScale {
+  static constexpr bool ON = std::is_same<T, XF16>::value;
+  static constexpr int TOP = 14;
+  float v = 1.f;
+  // dout: |dO|; square: of |V|
+  __device__ __forceinline__ void set(float dout, float square) {
+    const uint32_t e = (__float_as_uint(2.f * dout * sqrtf(square)) >> 23) & 255;
+    if (ON && e != 0 && e != 255) v = __uint_as_float((254 + TOP - e) << 23);
   }
-  return 1.f;
+  __device__ __forceinline__ float operator()(float ds) const { return ON ? ds * v : ds; }
+};
+
+// The squares of the largest |V| of the kept states, a chunk of them per block.
+// Bound by its launch, then by reading V once.  It adds to a backward: 2.5 us for
+// 64 x 32 states of 4 heads of 64 (of 29), 5 for 3 x 777 of 3 heads of 80 (of 60),
+// 7 for 4 x 1500 of 4 heads of 128 (of 266), 45 for 16 x 8192 of 8 (of 521).
+template <class T, int DP>
+__global__ __launch_bounds__(256) void xattn_vmax(const XArgs a) {
+  using I = Img<T, DP>;
+  using E = typename T::elem;
+  constexpr int LANES = I::CPR, ROWS = 256 / LANES;
+  __shared__ float top[4];
+  const int bh = blockIdx.x / a.chunks, c = blockIdx.x % a.chunks, b = bh / a.Hk;
+  const int lane = threadIdx.x % 64, ch = threadIdx.x % LANES;
+  const int len = a.kv_lens ? min(max(a.kv_lens[b], 0), a.Tk) : a.Tk;
+  const int per = (a.Tk + a.chunks - 1) / a.chunks;
+  const int hi = (int)min((long long)len, (c + 1LL) * per);
+  const E* V = (const E*)a.v.p + b * a.v.sb + bh % a.Hk * a.v.sh;
+  const uint8_t* mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+  float x = 0.f;
+#pragma unroll 4
+  for (int j0 = c * per; j0 < hi; j0 += ROWS) {
+    const int j = j0 + threadIdx.x / LANES;
+    const bool in = j < hi && (!mask || mask[j]) && ch * I::E < a.D;
+    const uint4 u = in ? ld_chunk<T>(V + j * a.v.st, ch, a.D) : zero16();
+    E e[I::E];
+    __builtin_memcpy(e, &u, 16);
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < I::E; ++i) s = fmaf(T::val(e[i]), T::val(e[i]), s);
+#pragma unroll
+    for (int m = 1; m < LANES; m <<= 1) s += __shfl_xor(s, m);
+    x = fmaxf(x, s);
+  }
+  x = wave_max(x);
+  if (lane == 0) top[threadIdx.x / 64] = x;
+  __syncthreads();
+  if (threadIdx.x == 0) a.vmax[blockIdx.x] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+// of all chunks of one key head, in every lane
+__device__ __forceinline__ float x_vmax(const XArgs& a, int bh) {
+  const int lane = threadIdx.x % 64;
+  return wave_max(lane < a.chunks ? a.vmax[(long long)bh * a.chunks + lane] : 0.f);
 }
 
-// dQ of WR * 32 rows, streaming K and V; also delta (and the rows' |dO|) for
+// dQ of WR * 32 rows, streaming K and V; also delta (and fp16's |dO|) for
 // xattn_dkv, which runs after it.  4 x 2048 rows on 2048 states, 16 heads of 128,
 // bf16: 194 us, 1061 TFLOP/s, bound by the matrix units.  fp32, 64 x 30 rows on
 // 196 states of 256: 20 us.
@@ -1075,7 +1128,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(c
 
   const int Dh = a.D - ds * S::DH;           // columns from this wave's first on
   Rows32<T, S::DH> qf, df;
-  float delta = 0.f, amax = 0.f;
+  float delta = 0.f, size = 0.f;
   {
     const bool live = row < rows;
     const E* o = live ? x_row<E>(a.o, w.b, w.g, a.G, row) + ds * S::DH : nullptr;
@@ -1092,12 +1145,16 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(c
 #pragma unroll
       for (int e = 0; e < I::E; ++e) {
         delta = fmaf(T::val(x[e]), T::val(y[e]), delta);
-        amax = fmaxf(amax, fabsf(T::val(x[e])));
+        if constexpr (DownScale<T>::ON) size = fmaf(T::val(x[e]), T::val(x[e]), size);
       }
     }
   }
   delta = xhalf_sum(delta);
-  amax = xhalf_max(amax);
+  DownScale<T> down;
+  if constexpr (DownScale<T>::ON) {
+    size = sqrtf(xhalf_sum(size));
+    down.set(size, x_vmax(a, w.bh));
+  }
   if constexpr (DS > 1) {                      // of all columns
     lds_stf(4 * (wave * 32 + lr), delta);
     __syncthreads();
@@ -1106,7 +1163,6 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(c
     __syncthreads();
   }
   const float L = row < rows ? a.lse[at + row] : INFINITY;
-  const float down = x_down<T>(amax);
   int turn = 0;
 
   auto masked = [&](f32x16 (&sp)[2], uint32_t kb) X_INLINE { x_mask(sp[0], kb, h); };
@@ -1170,13 +1226,12 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(c
   }
   if (w.split == 0 && ws == 0 && ds == 0 && h == 0 && row < a.R) {
     a.delta[at + row] = delta;
-    if (a.amax) a.amax[at + row] = amax;
+    if constexpr (DownScale<T>::ON) a.size[at + row] = size;
   }
   run(std::true_type{}, [&](f32x16 (&sp)[2], int e) X_INLINE {
-    sp[0][e] = probability(sp[0][e]) * (sp[1][e] - delta);
-    if constexpr (std::is_same<T, XF16>::value) sp[0][e] *= down;
+    sp[0][e] = down(probability(sp[0][e]) * (sp[1][e] - delta));
   });
-  const float mul = a.scale / down;
+  const float mul = a.scale / down.v;
   const bool none = L == INFINITY;
   const int tid = threadIdx.x % (64 * WR * WS);
   if (a.splits == 1) {
@@ -1235,15 +1290,15 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
   const float c2 = a.scale * LOG2E_X;
   const long long at = (long long)w.bh * a.R;
 
-  float down = 1.f;
-  if constexpr (std::is_same<T, XF16>::value) {
+  DownScale<T> down;
+  if constexpr (DownScale<T>::ON) {
     float x = 0.f;
-    for (int r = threadIdx.x; r < rows; r += C::NT) x = fmaxf(x, a.amax[at + r]);
+    for (int r = threadIdx.x; r < rows; r += C::NT) x = fmaxf(x, a.size[at + r]);
     x = wave_max(x);
     if (lane == 0) lds_stf(4 * wave, x);
     __syncthreads();
     for (int i = 0; i < C::NT / 64; ++i) x = fmaxf(x, lds_ldf(4 * i));
-    down = x_down<T>(x);
+    down.set(x, x_vmax(a, w.bh));
     __syncthreads();
   }
 
@@ -1285,8 +1340,7 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
     uint4 p[I::NPF], g[I::NPF];
     auto element = [&](int i) X_INLINE {
       sp[0][i] = __builtin_amdgcn_exp2f(fmaf(sp[0][i], c2, -L[i / 4][i % 4]));
-      sp[1][i] = sp[0][i] * (sp[1][i] - t[i / 4][i % 4]);
-      if constexpr (std::is_same<T, XF16>::value) sp[1][i] *= down;
+      sp[1][i] = down(sp[0][i] * (sp[1][i] - t[i / 4][i % 4]));
     };
     auto pack = [&](int c) X_INLINE {
       p[c] = I::pack(sp[0], c);
@@ -1482,7 +1536,7 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
         });
   }
   const int tid = threadIdx.x % (64 * WC * WS), Dh = min(a.D - ds * DH, DH);
-  const float mul = a.scale / down;
+  const float mul = a.scale / down.v;
   if (a.splits == 1) {
     const auto dst = [&](const XView& v) {
       return [&](int r) -> E* {
@@ -1593,6 +1647,14 @@ inline XPlan x_plan(const XArgs& a, int type, int what) {
   return p;
 }
 
+// Blocks for the largest |V| of a key head: 32 states or more each, no more than
+// 2048 in all where there are not more heads, at most one per lane of a wave.
+inline int x_chunks_of_v(const XArgs& a) {
+  const long long most = (a.Tk + 31) / 32, want = 2048 / ((long long)a.B * a.Hk);
+  const long long n = want < most ? want : most;
+  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
+
 template <class K>
 int x_go(K kernel, const XArgs& a, int lds, int nt, void* stream) {
   if (lds > 64 * 1024)
@@ -1641,6 +1703,10 @@ int x_run(XArgs a, int what, void* stream) {
   const XPlan p = x_plan(a, T::TYPE, what);
   a.tiles = p.tiles;
   a.splits = p.splits;
+  if constexpr (DownScale<T>::ON)
+    if (what == X_DQ)
+      hipLaunchKernelGGL((xattn_vmax<T, DP>), dim3((unsigned)(a.B * a.Hk * a.chunks)), dim3(256), 0,
+                         (hipStream_t)stream, a);
   const int e = x_waves<T, DP, 4>(a, p.waves, what, stream);
   if (e || a.splits == 1) return e;
   const dim3 grid((unsigned)(a.B * a.Hk * (what == X_DKV ? a.Tk : a.R)), what == X_DKV ? 2 : 1);

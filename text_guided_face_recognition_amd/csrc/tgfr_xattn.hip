@@ -79,7 +79,9 @@ int tgfr_cross_attention_ws(int B, int Tq, int Tk, int H, int Hk, int D, int typ
     else
       n = std::max({n, x_part(a, type, X_DQ), x_part(a, type, X_DKV)});
   }
-  *floats = n + (backward ? 2LL * B * Hk * a.R : 0);
+  if (backward)
+    n += (long long)B * Hk * (type == 2 ? 2LL * a.R + x_chunks_of_v(a) : a.R);
+  *floats = n;
   return 0;
 }
 
@@ -136,8 +138,13 @@ int tgfr_cross_attention_bwd(const void* q, const void* k, const void* v, const 
   a.scale = scale;
   a.lse = (float*)lse;
   a.delta = ws;
-  a.amax = type == 2 ? ws + (long long)B * Hk * a.R : nullptr;
-  a.part = ws + 2LL * B * Hk * a.R;
+  a.part = ws + (long long)B * Hk * a.R;
+  if (type == 2) {
+    a.chunks = x_chunks_of_v(a);
+    a.size = a.part;
+    a.vmax = a.size + (long long)B * Hk * a.R;
+    a.part = a.vmax + (long long)B * Hk * a.chunks;
+  }
   if (const int e = x_dispatch(a, type, X_DQ, stream)) return e;
   if (!dk) return 0;
   a.dk = view(dk, strides + 18);
