@@ -810,3 +810,22 @@ def test_attention_fp16_values_of_any_size(size, big, small):
     tol["dk"] = tol["dk"] + (scale * 2.0 ** -39 * per_head * rows).transpose(1, 2)
     for n, x in zip(("o", "dq", "dk", "dv"), (o.detach(), *grads)):
         within(x, want[n], tol[n], n)
+
+
+@pytest.mark.parametrize("tk", [8192, 131072, 524288])
+def test_attention_fp16_keeps_small_probabilities(tk):
+    """Even attention to many states: probabilities of 2^-13 to 2^-19 and the
+    dS made of them are operands in fp16, which has all its digits from 2^-14
+    on only.  dO is large, so that the gradients are in the type's range.  In
+    the 2-norm roundings of u / sqrt 3: 2 u, and 1e-4 for fp32 sums."""
+    b, tq, h, hk, d = 1, 40, 1, 1, 32
+    q, k, v, do, _ = inputs(F16, b, tq, tk, h, hk, d)
+    do = (do.float() * 256).to(F16)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = K.cross_attention(*leaves, scale=2.0 ** -5)
+    grads = torch.autograd.grad(o, leaves, do)
+    want, _ = formula(q, k, v, do, 2.0 ** -5, keep_of(b, tq, tk))
+    for n, x in zip(("o", "dq", "dk", "dv"), (o.detach(), *grads)):
+        floor = 2.0 ** -25 * math.sqrt(want[n].numel())
+        off = float((x.double() - want[n]).norm())
+        assert off <= (2 * half_step(F16) + 1e-4) * float(want[n].norm()) + floor, n

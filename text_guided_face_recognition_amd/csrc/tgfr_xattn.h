@@ -52,7 +52,7 @@ struct XArgs {
   const int* kv_lens;    // [B] or NULL
   const uint8_t* mask;   // [B][Tk], row stride mask_sb; nonzero: attended to; or NULL
   long long mask_sb;
-  float* lse;            // [B Hk][R]: log2 of the row's sum, in the log2 domain; +inf: none
+  float* lse;            // [B Hk][R]: log2 of the row's sum less T::PBITS; +inf: none
   float* delta;          // [B Hk][R]
   float* size;           // [B Hk][R] |dO| of the row (fp16 only)
   float* vmax;           // [B Hk][chunks] squares of the largest |V| (fp16 only)
@@ -66,7 +66,7 @@ struct XArgs {
 };
 
 struct XBf16 {
-  static constexpr int TYPE = 0, ES = 2;
+  static constexpr int TYPE = 0, ES = 2, PBITS = 0;
   using elem = uint16_t;
   static __device__ __forceinline__ f32x16 mma(uint4 a, uint4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(a), as_bf8(b), c, 0, 0, 0);
@@ -77,6 +77,9 @@ struct XBf16 {
 };
 struct XF16 {
   static constexpr int TYPE = 2, ES = 2;
+  // The backward's probabilities are held times 2^14: fp16 has all its digits from
+  // 2^-14 on only, and even attention to 2^19 states gives each 2^-19.
+  static constexpr int PBITS = 14;
   using elem = uint16_t;
   static __device__ __forceinline__ f32x16 mma(uint4 a, uint4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
@@ -91,7 +94,7 @@ struct XF16 {
   static __device__ __forceinline__ uint16_t bits(float x) { return f16_bits(x); }
 };
 struct XF32 {
-  static constexpr int TYPE = 1, ES = 4;
+  static constexpr int TYPE = 1, ES = 4, PBITS = 0;
   static constexpr bool VEC = true;       // rows of whole 16-byte chunks
   using elem = float;
   static __device__ __forceinline__ f32x16 mma(uint4 a, uint4 b, f32x16 c) {
@@ -984,7 +987,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(
   const long long at = (long long)w.bh * a.R;
   if (a.splits == 1) {
     if (a.lse && ws == 0 && ds == 0 && h == 0 && row < a.R)
-      a.lse[at + row] = none ? INFINITY : m + __builtin_amdgcn_logf(l);
+      a.lse[at + row] = none ? INFINITY : m + __builtin_amdgcn_logf(l) - T::PBITS;
     x_store<T, S::DH, WR, WS>(acc, mul / l, none, Dh, tid, ds * S::OUT, [&](int r) -> E* {
       return row0 + r < a.R ? x_row<E>(a.o, w.b, w.g, a.G, row0 + r) + ds * S::DH : nullptr;
     });
@@ -1035,7 +1038,7 @@ __global__ __launch_bounds__(256) void xattn_fwd_join(const XArgs a) {
     }
   }
   const bool none = m == -INFINITY && l == 0.f;
-  if (a.lse && d == 0) a.lse[id] = none ? INFINITY : m + __builtin_amdgcn_logf(l);
+  if (a.lse && d == 0) a.lse[id] = none ? INFINITY : m + __builtin_amdgcn_logf(l) - T::PBITS;
   if (d < a.D)
     x_row<E>(a.o, bh / a.Hk, bh % a.Hk, a.G, r)[d] = T::bits(none ? 0.f : o / l);
 }
@@ -1044,20 +1047,19 @@ __global__ __launch_bounds__(256) void xattn_fwd_join(const XArgs a) {
 // fp16 holds dS from 2^-24 to 2^16 only: dS is scaled by a power of two and the
 // sum scaled back in fp32.  |dP| and |delta| are at most |dO| |V| in the 2-norm, of
 // the row (for dK, whose sum runs over all rows, of the largest) and of the
-// largest kept state, so |dS| <= 2 |dO| |V| =: b as P <= 1.  The scale brings b to
-// [2^14, 2^15): nothing overflows, and dS keeps all of fp16's digits down to
-// 2^-28 b.  (Following the largest dP from piece to piece instead spares the
+// largest kept state, so |dS| <= 2 |dO| |V| =: b as P <= 1.  The scale and P's own
+// bring b to [2^14, 2^15): nothing overflows, and dS keeps all of fp16's digits
+// down to 2^-28 b.  (Following the largest dP from piece to piece instead spares the
 // launch below, but costs registers: backward of 4 x 2048 rows on 2048 states,
 // 16 heads of 128, 710 us against 541.)  bf16 and fp32 need none.
 template <class T>
 struct DownScale {
   static constexpr bool ON = std::is_same<T, XF16>::value;
-  static constexpr int TOP = 14;
   float v = 1.f;
   // dout: |dO|; square: of |V|
   __device__ __forceinline__ void set(float dout, float square) {
     const uint32_t e = (__float_as_uint(2.f * dout * sqrtf(square)) >> 23) & 255;
-    if (ON && e != 0 && e != 255) v = __uint_as_float((254 + TOP - e) << 23);
+    if (ON && e != 0 && e != 255) v = __uint_as_float((254 - e) << 23);
   }
   __device__ __forceinline__ float operator()(float ds) const { return ON ? ds * v : ds; }
 };
@@ -1202,9 +1204,10 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(c
       if constexpr (A && !B) x_exchange<DS>(next, ws * WR + wr, ds, turn);
     });
   };
-  auto probability = [&](float s) X_INLINE {
+  auto probability = [&](float s) X_INLINE {             // times 2^PBITS
     return __builtin_amdgcn_exp2f(fmaf(s, c2, -L));
   };
+  constexpr float POUT = 1.f / (1 << T::PBITS);
   // With few states, delta = sum P dP is summed from the products themselves:
   // dO . O carries the rounding of O to the type, which few states do not
   // average out (dQ was 1.53 times as far off as one rounding at 32 states,
@@ -1222,7 +1225,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(c
       sum = 0.f;
       for (int x = 0; x < WS; ++x) sum += lds_ldf(4 * ((x * WR + wr) * 32 + lr));
     }
-    if (L != INFINITY) delta = sum;
+    if (L != INFINITY) delta = sum * POUT;
   }
   if (w.split == 0 && ws == 0 && ds == 0 && h == 0 && row < a.R) {
     a.delta[at + row] = delta;
@@ -1231,7 +1234,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(c
   run(std::true_type{}, [&](f32x16 (&sp)[2], int e) X_INLINE {
     sp[0][e] = down(probability(sp[0][e]) * (sp[1][e] - delta));
   });
-  const float mul = a.scale / down.v;
+  const float mul = a.scale * POUT / down.v;
   const bool none = L == INFINITY;
   const int tid = threadIdx.x % (64 * WR * WS);
   if (a.splits == 1) {
@@ -1536,7 +1539,8 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
         });
   }
   const int tid = threadIdx.x % (64 * WC * WS), Dh = min(a.D - ds * DH, DH);
-  const float mul = a.scale / down.v;
+  constexpr float POUT = 1.f / (1 << T::PBITS);
+  const float mul = a.scale * POUT / down.v;
   if (a.splits == 1) {
     const auto dst = [&](const XView& v) {
       return [&](int r) -> E* {
@@ -1544,7 +1548,7 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
       };
     };
     x_store<T, DH, WC, WS>(dk, mul, !kept, Dh, tid, ds * C::OUT, dst(a.dk));
-    x_store<T, DH, WC, WS>(dv, 1.f, !kept, Dh, tid, ds * C::OUT, dst(a.dv));
+    x_store<T, DH, WC, WS>(dv, POUT, !kept, Dh, tid, ds * C::OUT, dst(a.dv));
   } else {
     const auto dst = [&](int which) {
       const long long ps =
@@ -1554,7 +1558,7 @@ __global__ __launch_bounds__(64 * WC * WS * DS) X_OCCUPANCY(OCC) void xattn_dkv(
       };
     };
     x_store<XF32, DH, WC, WS>(dk, mul, !kept, Dh, tid, ds * C::OUT32, dst(0));
-    x_store<XF32, DH, WC, WS>(dv, 1.f, !kept, Dh, tid, ds * C::OUT32, dst(1));
+    x_store<XF32, DH, WC, WS>(dv, POUT, !kept, Dh, tid, ds * C::OUT32, dst(1));
   }
 }
 
