@@ -829,3 +829,25 @@ def test_attention_fp16_keeps_small_probabilities(tk):
         floor = 2.0 ** -25 * math.sqrt(want[n].numel())
         off = float((x.double() - want[n]).norm())
         assert off <= (2 * half_step(F16) + 1e-4) * float(want[n].norm()) + floor, n
+
+
+def test_attention_fp16_many_faint_states():
+    """One state far above many others, each of which takes less than fp16's
+    smallest number beside it: together they are not nothing.  131071 states of
+    2^-25.2 of the first's probability, streamed by one block after it: off by
+    a half step of the result (2^-8.2) and by what fp16 drops of each, 2^-25 of
+    the scale that probabilities are held at, 2^11 or more of the largest:
+    2^17 2^-36; 2^-12 of it all for the exponents' fp32 error, 4 (64 + 8)
+    2^-24; and what the row's fp32 sum may lose beside its largest term, p."""
+    tq, tk, h, d = 2112, 131072, 3, 64
+    assert plan_floats((1, tq, tk, h, h, d), F16, 0) == 0
+    k = torch.zeros(1, tk, h, d, dtype=F16, device="cuda")
+    k[0, 5, :, 0] = 16.0
+    q = torch.zeros(1, tq, h, d, dtype=F16, device="cuda")
+    q[..., 0] = 1.0
+    v = torch.ones_like(k)
+    v[0, 5] = 0.0
+    p = (tk - 1) * 2.0 ** -25.2
+    want = p / (1.0 + p)
+    off = (K.cross_attention(q, k, v, scale=25.2 * math.log(2.0) / 16.0).double() - want).abs()
+    assert float(off.max()) <= want * (half_step(F16) + 2.0 ** -12 + p) + 2.0 ** -19

@@ -66,7 +66,7 @@ struct XArgs {
 };
 
 struct XBf16 {
-  static constexpr int TYPE = 0, ES = 2, PBITS = 0;
+  static constexpr int TYPE = 0, ES = 2, PBITS = 0, LAG = 8, UP = 0;
   using elem = uint16_t;
   static __device__ __forceinline__ f32x16 mma(uint4 a, uint4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(a), as_bf8(b), c, 0, 0, 0);
@@ -80,6 +80,9 @@ struct XF16 {
   // The backward's probabilities are held times 2^14: fp16 has all its digits from
   // 2^-14 on only, and even attention to 2^19 states gives each 2^-19.
   static constexpr int PBITS = 14;
+  // The forward's, relative to the running maximum, stay below 2^(LAG + UP) and
+  // begin to lose digits at 2^(-14 - UP): many states far below one count.
+  static constexpr int LAG = 4, UP = 11;
   using elem = uint16_t;
   static __device__ __forceinline__ f32x16 mma(uint4 a, uint4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
@@ -94,7 +97,7 @@ struct XF16 {
   static __device__ __forceinline__ uint16_t bits(float x) { return f16_bits(x); }
 };
 struct XF32 {
-  static constexpr int TYPE = 1, ES = 4, PBITS = 0;
+  static constexpr int TYPE = 1, ES = 4, PBITS = 0, LAG = 8, UP = 0;
   static constexpr bool VEC = true;       // rows of whole 16-byte chunks
   using elem = float;
   static __device__ __forceinline__ f32x16 mma(uint4 a, uint4 b, f32x16 c) {
@@ -907,8 +910,8 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(
   int turn = 0;
   // the reference that exponents are taken against, in the log2 domain:
   // exp(scale s - max) = 2^(c2 s - m).  It follows the running maximum only
-  // once that has grown by 8: sums and accumulators, relative to it, stay
-  // exact, probabilities stay below 2^8, and most tiles rescale nothing.
+  // once that has grown by LAG: sums and accumulators, relative to it, stay
+  // exact, probabilities stay below 2^LAG, and most tiles rescale nothing.
   float m = -INFINITY, l = 0.f;
 
   auto before = [&](f32x16 (&sp)[1], uint32_t kb) X_INLINE {
@@ -918,7 +921,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(
 #pragma unroll
     for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
     top = xhalf_max(top) * c2;
-    if (__any(top > m + 8.f || m == -INFINITY)) {
+    if (__any(top > m + T::LAG || m == -INFINITY)) {
       const float mn = fmaxf(m, top);
       const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
@@ -932,7 +935,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(
              f32x16 (&next)[1], const auto& kn, const auto&) X_INLINE {
     constexpr bool A = first.value, B = rest.value;
     constexpr int RM = A ? I::NC : 0, TR = B ? I::NPF * NB : 0, PER = 16 / I::NC;
-    const float mu = m == -INFINITY ? 0.f : m;        // no kept state so far
+    const float mu = m == -INFINITY ? 0.f : m - T::UP;        // no kept state so far
     uint4 p[I::NPF];
     auto probability = [&](int e) X_INLINE {
       sp[0][e] = __builtin_amdgcn_exp2f(fmaf(sp[0][e], c2, -mu));
@@ -962,6 +965,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(
     if constexpr (A && !B) x_exchange<DS>(next, ws * WR + wr, ds, turn);
   });
   l = xhalf_sum(l);
+  m -= T::UP;                   // what l and acc are relative to
 
   float mul = 1.f;
   if constexpr (WS > 1) {       // the waves that share rows agree on the reference
