@@ -851,3 +851,24 @@ def test_attention_fp16_many_faint_states():
     want = p / (1.0 + p)
     off = (K.cross_attention(q, k, v, scale=25.2 * math.log(2.0) / 16.0).double() - want).abs()
     assert float(off.max()) <= want * (half_step(F16) + 2.0 ** -12 + p) + 2.0 ** -19
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_attention_strides_of_axes_of_one(dtype):
+    """The stride of an axis of one token, head or sample means nothing."""
+    far = 1 << 40
+    q, k, v, do, _ = inputs(dtype, 1, 1, 1, 1, 1, 64)
+    want = check(q, k, v, do)
+    x = [t.as_strided(t.shape, (far, far, far, 1)) for t in (q, k, v, do)]
+    got = [t.detach().requires_grad_() for t in x[:3]]
+    o = K.cross_attention(*got)
+    assert torch.equal(o, want[0])
+    for a, c in zip(torch.autograd.grad(o, got, x[3]), want[1]):
+        assert torch.equal(a, c)
+    q, k, v, do, _ = inputs(dtype, 3, 1, 50, 4, 2, 64)
+    want = check(q, k, v, do)
+    one = q.as_strided(q.shape, (q.stride(0), far, 64, 1)).detach().requires_grad_()
+    o = K.cross_attention(one, k, v)
+    assert torch.equal(o, want[0])
+    assert torch.equal(torch.autograd.grad(o, one, do.as_strided(do.shape, one.stride()))[0],
+                       want[1][0])

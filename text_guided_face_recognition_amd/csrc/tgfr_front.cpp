@@ -89,12 +89,15 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor dense(const Tensor& t) {
   return !t.defined() || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
 }
+// (that of an axis of one means nothing and may be anything)
+int64_t stride(const Tensor& t, int axis) { return t.size(axis) == 1 ? 0 : t.stride(axis); }
 // the kernels reach the rows of a tile by 32-bit offsets: tensors whose tokens
 // (or shared heads) lie further apart are copied
 Tensor near(const Tensor& t, int64_t heads) {
   const Tensor d = dense(t);
   const int64_t size = (int64_t)d.element_size();
-  return (160 * d.stride(1) + heads * d.stride(2) + 256) * size < (1LL << 31) ? d : d.contiguous();
+  return (160 * stride(d, 1) + heads * stride(d, 2) + 256) * size < (1LL << 31) ? d
+                                                                              : d.contiguous();
 }
 Tensor floats(int64_t n, const Tensor& like) {
   return at::empty({n}, like.options().dtype(at::kFloat).requires_grad(false));
@@ -148,7 +151,7 @@ struct Attn {
   int64_t mask_sb() const { return mask.defined() ? mask.stride(0) : 0; }
 };
 int64_t* strides(int64_t* s, const Tensor& t) {
-  for (int i = 0; i < 3; ++i) *s++ = t.stride(i);
+  for (int i = 0; i < 3; ++i) *s++ = stride(t, i);
   return s;
 }
 
