@@ -820,6 +820,8 @@ int tgfr_fcfm_conv_dw(const float* x, long long s_b, long long s_p, const float*
  *   type: 0 = bf16, 1 = fp32, 2 = fp16 tensors.
  *   strides (host memory): 3 per tensor, over samples, tokens and heads, in
  * elements, in the order of the tensor arguments; the last axis is dense.
+ * At most 2^30 rows of queries, and of keys, of all heads and samples, and
+ * 2^24 - 1 key heads of all samples (1001).
  * Any alignment of the element is read and written.  160 times the token
  * stride plus H / Hk times the head stride, of q, k, v and dout, stay below
  * 2^31 bytes (1001): tiles are read by 32-bit offsets from their first row.

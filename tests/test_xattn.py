@@ -47,6 +47,18 @@ def test_cross_attention_refuses_too_many_rows():
         K.cross_attention(x, torch.zeros(1, 1, 1, 1), torch.zeros(1, 1, 1, 1))
 
 
+def test_cross_attention_refuses_too_many_key_heads():
+    """A launch has at most 2^32 - 1 threads, and a key head 256 or more."""
+    x = torch.zeros(1, 1, 1, 1).expand(1 << 24, 1, 1, 1)
+    with pytest.raises(ValueError):
+        K.cross_attention(x, x, x)
+    n = ctypes.c_longlong(0)
+    for b, ok in ((1 << 24, 1001), ((1 << 24) - 1, 0)):
+        for backward in (0, 1):
+            assert _hip.lib().tgfr_cross_attention_ws(b, 1, 1, 1, 1, 64, 0, backward,
+                                                      ctypes.byref(n)) == ok
+
+
 def norm_args(d=16, dtype=torch.float32):
     return dict(q=torch.zeros(2, 5, 4, d, dtype=dtype), k=torch.zeros(2, 7, 2, d, dtype=dtype),
                 q_weight=torch.ones(d), k_weight=torch.ones(d),

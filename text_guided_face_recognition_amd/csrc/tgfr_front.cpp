@@ -256,6 +256,7 @@ py::object cross_attention(py::handle hq, py::handle hk, py::handle hv, py::hand
   if (a.tq > most || a.tk > most || a.b > most || a.h > most ||
       (double)a.b * a.h * std::max(a.tq, a.tk) > (double)most)
     bad_value("at most 2^30 rows of queries or keys");
+  if (a.b * a.hk >= 1LL << 24) bad_value("at most 2^24 - 1 key heads of all samples");
   const double scale = hscale.is_none() ? 1.0 / std::sqrt((double)a.d) : hscale.cast<double>();
   if (!((float)scale > 0.f) || std::isinf((float)scale))
     bad_value("scale must be positive and finite, got ", scale);

@@ -1663,11 +1663,15 @@ inline int x_chunks_of_v(const XArgs& a) {
   return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 
+// threads of a launch
+constexpr long long X_THREADS = 0xffffffffLL;
+
 template <class K>
 int x_go(K kernel, const XArgs& a, int lds, int nt, void* stream) {
   if (lds > 64 * 1024)
     if (const int e = set_max_lds((const void*)kernel, lds)) return e;
   const long long grid = (long long)a.tiles * a.splits * a.B * a.Hk;
+  if (grid * nt > X_THREADS) return 1001;
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(nt), lds, (hipStream_t)stream, a);
   return (int)hipGetLastError();
 }

@@ -18,7 +18,9 @@ int x_shape(XArgs& a, int type, int B, int Tq, int Tk, int H, int Hk, int D) {
   if (B < 1 || Tq < 1 || Tk < 1 || H < 1 || Hk < 1 || H % Hk || D < 1 || D > 256) return 1001;
   // row and state numbers, and the grids (one block or wave per row), are 32-bit
   const long long rows = (long long)Tq * (H / Hk), lim = 1LL << 30;
-  if (H / Hk > 32768 || rows > lim || Tk > lim || rows * B * Hk > lim || (long long)Tk * B * Hk > lim) return 1001;
+  if (H / Hk > 32768 || rows > lim || Tk > lim || rows * B * Hk > lim ||
+      (long long)Tk * B * Hk > lim || (long long)B * Hk * 256 > X_THREADS)
+    return 1001;
   a.B = B;
   a.Tq = Tq;
   a.Tk = Tk;
