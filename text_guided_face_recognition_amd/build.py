@@ -6,7 +6,7 @@ tgfr_front.so, the compiled torch front-end of some of its entries.
 Each csrc/*.hip compiles to its own object (in parallel, with per-file
 flags), then hipcc links the shared library, which does not depend on torch.
 csrc/tgfr_front.cpp (host code against torch's headers) is a Python module of
-its own beside it.
+its own beside it, left out where torch is not installed.
 
 The library is stamped with a hash of everything it is built from (sources,
 headers, this file's flags): ``stale()`` compares the stamp with the tree, and
@@ -61,11 +61,15 @@ def deps():
 
 
 def torch_dir():
-    """torch's folder, found without importing it."""
-    return importlib.util.find_spec("torch").submodule_search_locations[0]
+    """torch's folder, found without importing it; None where there is none
+    (the library is built for other hosts then, without the front-end)."""
+    spec = importlib.util.find_spec("torch")
+    return spec and spec.submodule_search_locations[0]
 
 
 def torch_version():
+    if torch_dir() is None:
+        return "none"
     with open(os.path.join(torch_dir(), "version.py")) as f:
         return f.read()
 
@@ -95,7 +99,7 @@ def source_hash(extra=()):
 
 def stale():
     """True when the library is missing or was built from other sources."""
-    if not all(os.path.exists(p) for p in (LIB, FRONT, STAMP)):
+    if not all(os.path.exists(p) for p in (LIB, STAMP) + (FRONT,) * (torch_dir() is not None)):
         return True
     with open(STAMP) as f:
         return f.read().strip() != source_hash()
@@ -141,7 +145,9 @@ def _build_locked(verbose, extra):
         jobs.append(([*common, *FILE_FLAGS.get(name, []), "-c", src, "-o", obj], obj))
     # the files that take longest first
     jobs.sort(key=lambda j: -os.path.getsize(j[0][-3]) - 10**6 * ("xattn_" in j[1]))
-    jobs.append((front_command(), None))
+    front = torch_dir() is not None
+    if front:
+        jobs.append((front_command(), None))
     workers = max(1, min(len(jobs), int(os.environ.get("MAX_JOBS", os.cpu_count() or 4))))
     with ThreadPoolExecutor(workers) as ex:
         list(ex.map(lambda j: _run(j[0], verbose), jobs))
@@ -149,7 +155,8 @@ def _build_locked(verbose, extra):
     _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-fno-gpu-rdc", "-o", tmp,
           *sorted(o for _, o in jobs if o)], verbose)
     os.replace(tmp, LIB)
-    os.replace(FRONT + ".tmp", FRONT)
+    if front:
+        os.replace(FRONT + ".tmp", FRONT)
     with open(STAMP, "w") as f:
         f.write(digest + "\n")
     return LIB
