@@ -872,3 +872,83 @@ def test_attention_strides_of_axes_of_one(dtype):
     assert torch.equal(o, want[0])
     assert torch.equal(torch.autograd.grad(o, one, do.as_strided(do.shape, one.stride()))[0],
                        want[1][0])
+
+
+def test_views_that_negate():
+    """The imaginary part of a conjugate is a view that negates what it holds."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+
+    def pair(*shape):
+        x = randn(g, *shape, dtype=F32)
+        view = torch.complex(torch.zeros_like(x), -x).conj().imag
+        assert view.is_neg() and torch.equal(view, x)
+        return x, view
+    (q, qn), (do, don) = pair(2, 5, 4, 16), pair(2, 5, 4, 16)
+    (k, kn), (v, vn), (w, wn) = pair(2, 9, 2, 16), pair(2, 9, 2, 16), pair(16)
+    leaves, views = ([x.detach().requires_grad_() for x in t]
+                     for t in ((q, k, v, w), (qn, kn, vn, wn)))
+    rope, runs = K.Rope(16), []
+    for a, d in ((leaves, do), (views, don)):
+        y = K.qk_norm_rope(a[0], a[1], a[3], a[3], rope=rope)
+        o = K.cross_attention(a[0], a[1], a[2])
+        runs.append([*y, o, *torch.autograd.grad((o, y[0]), a, (d, d))])
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
+
+
+def test_norm_of_both_with_one_used():
+    """A part whose result no loss uses has zero gradients, the other its own."""
+    g = torch.Generator(device="cuda").manual_seed(13)
+    x = [randn(g, 2, 5, 4, 16, dtype=F32), randn(g, 2, 9, 2, 16, dtype=F32),
+         randn(g, 16, dtype=F32), randn(g, 16, dtype=F32)]
+    dy = [randn(g, *t.shape, dtype=F32) for t in x[:2]]
+    x = [t.requires_grad_() for t in x]
+    rope = K.Rope(16)
+    for i in range(2):
+        y = K.qk_norm_rope(*x, rope=rope)
+        got = torch.autograd.grad(y[i], x, dy[i], allow_unused=True)
+        alone = [x[i], x[2 + i]]
+        z = K.qk_norm_rope(*([x[0], None, x[2], None] if i == 0 else [None, x[1], None, x[3]]),
+                           rope=rope)[i]
+        want = torch.autograd.grad(z, alone, dy[i])
+        assert torch.equal(got[i], want[0])
+        # (sums of dw run over other numbers of blocks)
+        within(got[2 + i], want[1].double(), 64 * U32 * want[1].abs().double() + 1e-4, "dw")
+        for t in (got[1 - i], got[3 - i]):
+            assert t is None or not t.any()
+
+
+@pytest.mark.parametrize("dtype", [BF, F16], ids=["bf16", "fp16"])
+def test_attention_two_graphs_and_two_streams(dtype):
+    """Two graphs captured from one pool, replayed in turn and between eager
+    calls on two streams at once: every result is the eager one's."""
+    data = [inputs(dtype, 2, 40 + i, 700, 4, 2, 64, seed=i)[:4] for i in range(2)]
+
+    def step(q, k, v, do):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = K.cross_attention(*leaves)
+        return [o.detach(), *torch.autograd.grad(o, leaves, do)]
+    eager = [step(*x) for x in data]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    pool = torch.cuda.graph_pool_handle()
+    for x in data:
+        with torch.cuda.stream(streams[0]):
+            step(*x)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], pool=pool):
+            outs.append(step(*x))
+    for turn in range(3):
+        for i in (turn % 2, 1 - turn % 2):
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs[i], eager[i]))
+        both = []
+        for s, x in zip(streams, data):
+            with torch.cuda.stream(s):
+                both.append(step(*x))
+        torch.cuda.synchronize()
+        for got, want in zip(both, eager):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
