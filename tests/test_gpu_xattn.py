@@ -200,6 +200,17 @@ def test_attention_many_samples_states_and_heads(dtype, size):
     check(*x, kv_lens=kv_lens, mask=mask)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("b", [512, 513])
+def test_attention_lengths_of_many_samples(dtype, b):
+    """Either side of the batch from which tiles of padding are not put last."""
+    tq, tk = 130, 150
+    *x, g = inputs(dtype, b, tq, tk, 2, 1, 64)
+    q_lens = torch.randint(0, tq + 1, (b,), generator=g, device="cuda")
+    kv_lens = torch.randint(0, tk + 1, (b,), generator=g, device="cuda")
+    check(*x, q_lens=q_lens, kv_lens=kv_lens)
+
+
 def test_attention_lengths_of_any_size():
     """64-bit lengths are clamped, not wrapped, on the way to 32 bits."""
     q, k, v, _, _ = inputs(F32, 4, 6, 40, 2, 1, 64)
