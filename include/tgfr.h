@@ -35,6 +35,8 @@
  *   - ABI 610: tgfr_imim_dw_ln; tgfr_ln_tail_bwd / _att accept dlnw = dlnb =
  *     NULL (the LayerNorm's dw / db partials stay in ws for it).
  *   - ABI 620: tgfr_ln_tail_bwd_att keeps dZ in bf16 (half the scratch).
+ *     tgfr_cross_attention_* and tgfr_qk_norm_rope_* joined under this number
+ *     (additions only): a host that may meet an older library looks them up.
  */
 #ifndef TGFR_H
 #define TGFR_H

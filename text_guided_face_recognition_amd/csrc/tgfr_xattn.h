@@ -21,8 +21,9 @@
 //
 // fp32 runs on v_mfma_f32_32x32x2_f32 (every product and sum in 32 bits).
 // bf16 / fp16 round P and dS to the type as MFMA operands (2^-8 / 2^-11
-// relative, of the size of the one rounding of the result); sums, statistics
-// and accumulators are fp32.
+// relative, of the size of the one rounding of the result), fp16 scaled by powers
+// of two into its range (XF16, DownScale); sums, statistics and accumulators are
+// fp32.
 //
 // Masked states never reach a product: their rows of K and V are written to
 // LDS as zeros (NaN or infinity there stays there) and their scores are -inf.
@@ -297,7 +298,11 @@ struct Feed {
              base + wave + 16 * NT * n);
   }
   // the same for rows at any alignment and of any length, through registers:
-  // at(i) points to row i of the tile, or is NULL for zeros
+  // at(i) points to row i of the tile, or is NULL for zeros.  No tile is fed
+  // beside another's work here (16 heads of 128 on 4, 4 x 1024 x 1500, forward /
+  // backward: rows at 2 bytes 114 / 724 us, at 4 bytes or more 60 / 236; 100
+  // columns 132 / 827, 104 columns 57 / 230; 12 heads on 4, whose groups of 3
+  // straddle tiles in dK and dV alone, 50 / 452, on 6 50 / 208)
   template <class Row>
   __device__ __forceinline__ void copy(Row at, int D, uint32_t base) const {
 #pragma unroll
@@ -889,7 +894,9 @@ __device__ __forceinline__ void x_mask(f32x16& s, uint32_t kb, int h) {
 // TFLOP/s, bound by the matrix units (a library product of 8192^3: 1172).  One
 // token, 16 samples, 32 heads on 8, up to 8192 states: 72 us, 4.8 TB/s, bound by
 // reading K and V.  fp32, 64 x 30 rows on 196 states of 256: 15 us, bound by the
-// latency of its 4 splits' two pieces.
+// latency of its 4 splits' two pieces; 4 x 1024 rows of 16 heads of 128 on 4 x 1500
+// states of 4: 473 us, 106 TFLOP/s of 153; one token, 16 samples, 32 heads on 8, 8192
+// states: 226 us, 4.7 TB/s.
 template <class T, int DP, int WR, int WS, int DS, int OCC>
 __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(const XArgs a) {
   using S = KeyStream<T, DP, WR, WS, DS, true>;
@@ -1266,7 +1273,8 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_dq(c
 // 4 x 2048 rows on 2048 states, 16 heads of 128, bf16: 290 us, 946 TFLOP/s.
 // A wave of 128 columns is alone on its SIMD and issues 320 instructions a
 // piece in the time of 32 matrix instructions and half as long again: bound by
-// issue.  fp32, 64 x 30 rows on 196 states of 256: 26 us, 65 TFLOP/s.
+// issue.  fp32, 64 x 30 rows on 196 states of 256: 26 us, 30 TFLOP/s (36 with the
+// rows that fill the last pieces).
 template <class T, int DP, int WC, int WS, int DS>
 struct DkvCfg {
   static constexpr int NT = 64 * WC * WS * DS, RT = 32 * WS;
@@ -1630,8 +1638,8 @@ constexpr int x_least(int type, int what, int dp) {
 // heads on 8: 101 us against 142; without a mask 84 against 77).  What still leaves
 // CUs without a block splits the stream over blocks, 128 items (fp32: 64) or
 // more each and no more blocks than run at once; a second launch joins them
-// (17 tokens of 8 heads on 8192 states: 32 us against 114; not at 99 blocks: 22
-// both ways; 4 x 5 x 1500, 12 heads of 64, masked: 14.4 us in one round of 480
+// (17 tokens of 8 heads on 8192 states: 32 us against 114; not at 99 blocks, 3 x
+// 333 x 777, 6 heads of 80 on 3, masked: 31 us both ways; 4 x 5 x 1500, 12 heads of 64, masked: 14.4 us in one round of 480
 // blocks, 21.7 in one and an eighth of 256; 64 x 30 x 196 of 256, fp32: 21.2 us by 4
 // splits, 23.0 by 7).
 inline XPlan x_plan(const XArgs& a, int type, int what) {

@@ -2237,8 +2237,8 @@ def cross_attention(q, k, v, scale=None, q_lens=None, kv_lens=None, mask=None):
     the whole card.
 
     Sums, softmax statistics and accumulators are fp32; bf16 / fp16 round the
-    probabilities (backward: dS) to the type as matrix operands.  Equal calls
-    give equal bits.  Only enqueues work on the current stream of q's device:
+    probabilities (backward: dS) to the type as matrix operands, fp16 scaled
+    into its range.  Equal calls give equal bits.  Only enqueues work on the current stream of q's device:
     can be captured into a HIP graph, a backward together with its forward
     (autograd runs a backward on its forward's stream, so one whose forward
     ran eagerly does not belong into a capture).  Second derivatives,
