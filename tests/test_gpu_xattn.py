@@ -963,3 +963,29 @@ def test_attention_two_graphs_and_two_streams(dtype):
         torch.cuda.synchronize()
         for got, want in zip(both, eager):
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -4, 0.25, 1.0, 2.0, 4.0])
+@pytest.mark.parametrize("dtype", [BF, F16, F32], ids=["bf16", "fp16", "fp32"])
+def test_attention_scores_in_the_millions(dtype, scale):
+    """Scores of 2^21 to 2^27: a row whose best state is ahead of the others by
+    more than the scores' error, (64 + 8) 2^-24 of their magnitudes, is that
+    state's V, off by the roundings of its probability and of the result: 2 u,
+    and 40 2^-24 of fp32 arithmetic.  (Gradients of such rows hang on exponents
+    that fp32 does not hold: finite.)"""
+    q, k, v, do, _ = inputs(dtype, 2, 40, 200, 2, 2, 64)
+    q, k = (1024 * q.float()).to(dtype), (1024 * k.float()).to(dtype)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = K.cross_attention(*leaves, scale=scale)
+    for t in (o, *torch.autograd.grad(o, leaves, do)):
+        assert bool(torch.isfinite(t).all())
+    o = o.detach()
+    Q, KK = heads(q, 2), heads(k, 2)
+    s = scale * Q @ KK.transpose(2, 3)
+    err = 72 * U32 * scale * (Q.abs() @ KK.abs().transpose(2, 3)).amax(-1)
+    top = s.topk(2, -1)
+    sure = top.values[..., 0] - top.values[..., 1] > 2 * err + 100
+    assert float(sure.double().mean()) > 0.9
+    want = torch.gather(heads(v, 2), 2, top.indices[..., :1].expand(-1, -1, -1, 64))
+    off = (o.double().transpose(1, 2) - want).abs() - (2 * half_step(dtype) + 40 * U32) * want.abs()
+    assert float(off[sure].max()) <= 0

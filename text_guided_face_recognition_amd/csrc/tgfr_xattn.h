@@ -889,6 +889,14 @@ __device__ __forceinline__ void x_mask(f32x16& s, uint32_t kb, int h) {
   }
 }
 
+// A row's statistic for the backward.  Past 2^22, where fp32's steps make exponents
+// inexact by 2^-2 and more, fp16 takes it a step high: P stays in the type.
+template <class T>
+__device__ __forceinline__ float x_lse(float m, float l) {
+  const float x = m + __builtin_amdgcn_logf(l) - T::PBITS;
+  return T::PBITS && fabsf(x) >= 0x1p22f ? fmaf(fabsf(x), 0x1p-23f, x) : x;
+}
+
 // ------------------------------------------------------------------ forward ---
 // 4 x 2048 rows of 16 heads of 128 on 4 x 4096 states of 4, bf16: 261 us, 1050
 // TFLOP/s, bound by the matrix units (a library product of 8192^3: 1172).  One
@@ -922,7 +930,11 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(
   // the reference that exponents are taken against, in the log2 domain:
   // exp(scale s - max) = 2^(c2 s - m).  It follows the running maximum only
   // once that has grown by LAG: sums and accumulators, relative to it, stay
-  // exact, probabilities stay below 2^LAG, and most tiles rescale nothing.
+  // exact, probabilities stay below 2^(LAG + UP), and most tiles rescale nothing.
+  // (Past 2^22 the fp32 steps of m would take the place of UP: it is left out.)
+  auto reference = [&](float top) X_INLINE {
+    return T::UP && fabsf(top) < 0x1p22f ? top - T::UP : top;
+  };
   float m = -INFINITY, l = 0.f;
 
   auto before = [&](f32x16 (&sp)[1], uint32_t kb) X_INLINE {
@@ -931,7 +943,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(
     float top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
-    top = xhalf_max(top) * c2;
+    top = reference(xhalf_max(top) * c2);
     if (__any(top > m + T::LAG || m == -INFINITY)) {
       const float mn = fmaxf(m, top);
       const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
@@ -946,7 +958,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(
              f32x16 (&next)[1], const auto& kn, const auto&) X_INLINE {
     constexpr bool A = first.value, B = rest.value;
     constexpr int RM = A ? I::NC : 0, TR = B ? I::NPF * NB : 0, PER = 16 / I::NC;
-    const float mu = m == -INFINITY ? 0.f : m - T::UP;        // no kept state so far
+    const float mu = m == -INFINITY ? 0.f : m;        // no kept state so far
     uint4 p[I::NPF];
     auto probability = [&](int e) X_INLINE {
       sp[0][e] = __builtin_amdgcn_exp2f(fmaf(sp[0][e], c2, -mu));
@@ -976,7 +988,6 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(
     if constexpr (A && !B) x_exchange<DS>(next, ws * WR + wr, ds, turn);
   });
   l = xhalf_sum(l);
-  m -= T::UP;                   // what l and acc are relative to
 
   float mul = 1.f;
   if constexpr (WS > 1) {       // the waves that share rows agree on the reference
@@ -1002,7 +1013,7 @@ __global__ __launch_bounds__(64 * WR * WS * DS) X_OCCUPANCY(OCC) void xattn_fwd(
   const long long at = (long long)w.bh * a.R;
   if (a.splits == 1) {
     if (a.lse && ws == 0 && ds == 0 && h == 0 && row < a.R)
-      a.lse[at + row] = none ? INFINITY : m + __builtin_amdgcn_logf(l) - T::PBITS;
+      a.lse[at + row] = none ? INFINITY : x_lse<T>(m, l);
     x_store<T, S::DH, WR, WS>(acc, mul / l, none, Dh, tid, ds * S::OUT, [&](int r) -> E* {
       return row0 + r < a.R ? x_row<E>(a.o, w.b, w.g, a.G, row0 + r) + ds * S::DH : nullptr;
     });
@@ -1053,7 +1064,7 @@ __global__ __launch_bounds__(256) void xattn_fwd_join(const XArgs a) {
     }
   }
   const bool none = m == -INFINITY && l == 0.f;
-  if (a.lse && d == 0) a.lse[id] = none ? INFINITY : m + __builtin_amdgcn_logf(l) - T::PBITS;
+  if (a.lse && d == 0) a.lse[id] = none ? INFINITY : x_lse<T>(m, l);
   if (d < a.D)
     x_row<E>(a.o, bh / a.Hk, bh % a.Hk, a.G, r)[d] = T::bits(none ? 0.f : o / l);
 }
